@@ -640,6 +640,52 @@ psb_status psb_sign_search_candidates(int mode, const float* d_states, const flo
                                       int padded_dim, int candidate_count, int* d_rows_out, float* d_dist_out, int device,
                                       void* stream);
 
+/* ---- rows of 8-bit codes: encoding, norm, products ------------------------------------------------------------
+ * Rows held as signed 8-bit codes with one fp32 scale a row, value = code * scale: stored rows that are scored by inner products, and a
+ * generating model's weights and activations.  No counterpart in the reference (its 8-bit rows are the caller's own u8 values).  All pointers
+ * are DEVICE pointers on `device`; the calls are asynchronous on `stream`, allocate nothing, can be captured, and leave the current device as
+ * it was.  Strides are in elements.  Outputs may not lie over other arrays unless said so.  Rows and columns behind the last are not written. */
+enum { PSB_TYPE_F32 = 0, PSB_TYPE_F16 = 1, PSB_TYPE_BF16 = 2 };
+
+/* code = rint(127 x / max|x|), ties to even, as in 64-bit arithmetic; scale = max|x| / 127.  A row of zeros has scale 0; one with an infinity
+ * or a NaN has codes 0 and scale NaN.  n >= 0 rows of 1 <= dim <= 131,071 elements of `type`.  psb_i8_matmul wants d_codes at a multiple of 16
+ * bytes and code_stride a multiple of 16. */
+psb_status psb_i8_encode_rows(const void* d_rows, int type, int64_t n, int dim, int64_t row_stride, int8_t* d_codes, int64_t code_stride,
+                              float* d_scales, int device, void* stream);
+/* Root-mean-square norm of x + residual to codes: h = x + residual (d_residual may be NULL), u = h * weight (d_weight [dim] of `type`; NULL =
+ * ones), code = rint(127 u / max|u|) as above, scale = max|u| / (127 sqrt(mean(h^2) + eps)), so that code * scale is u / rms.  d_sum (may be
+ * NULL) receives h rounded to `type`; it may be d_rows or d_residual themselves, with the same stride.  The norm is of the unrounded h. */
+psb_status psb_i8_norm_rows(const void* d_rows, const void* d_residual, const void* d_weight, int type, int64_t n, int dim, int64_t row_stride,
+                            int64_t residual_stride, float eps, void* d_sum, int64_t sum_stride, int8_t* d_codes, int64_t code_stride,
+                            float* d_scales, int device, void* stream);
+/* out[i][j] = x_scale[i] * w_scale[j] * sum_k x[i][k] * w[j][k] for m rows x (tokens, queries) and n rows w (output channels, stored rows) of k
+ * codes, 1 <= k <= 131,071.  The sums are exact; ((float)sum * x_scale) * w_scale in fp32, rounded to out_type.  Rows of codes begin at multiples
+ * of 16 bytes (pointers and strides); out [m][out_stride]. */
+psb_status psb_i8_matmul(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride,
+                         const float* d_w_scales, int64_t n, int k, void* d_out, int out_type, int64_t out_stride, int device, void* stream);
+/* Test hook of its time-out path: only the first `tiles` output tiles (-1: all) get their products from the tensor cores, waits end after `polls`.
+ * A block that waits in vain forms its outputs without them, so that the results are the same. */
+psb_status psb_i8_matmul_limited(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride,
+                                 const float* d_w_scales, int64_t n, int k, void* d_out, int out_type, int64_t out_stride, int64_t tiles, int polls,
+                                 int device, void* stream);
+
+/* ---- beams: selection over beams and vocabulary, states in the new order ------------------------------------------
+ * No counterpart in the reference.  Pointers, streams and devices as for rows of codes. */
+
+/* The k best continuations of each of `batch` items over its beams and the vocabulary: total = d_scores[item][beam] + log p(token), log p the
+ * log-softmax of the beam's logits (d_logits [batch * beams][row_stride] of `type`), largest first, ties to the lowest (beam, token).  A token
+ * with logit -inf is never chosen; neither is one of a beam whose score is not finite or whose logits hold a NaN or +inf or nothing but -inf.
+ * d_parents, d_tokens [batch][k] int32 (-1 where fewer are left), d_totals [batch][k] fp32 (-inf there).  beams <= 64, k <= 64,
+ * vocab <= 2^24, batch <= 2^20. */
+psb_status psb_beam_select(const void* d_logits, int type, int64_t row_stride, const float* d_scores, int batch, int beams, int vocab, int k,
+                           int* d_parents, int* d_tokens, float* d_totals, int device, void* stream);
+/* States [layers][batch][beams][heads][tokens][token_bytes] brought into the new order: out[.., item, j, ..] = in[.., item, parent[item][j], ..]
+ * for the first d_lengths[item] tokens (NULL: all); what lies behind them is left as it was, and so is a beam whose parent is outside
+ * 0..beams-1.  d_out is d_in (any parents: the states are reordered where they are) or does not overlap it.  d_parents [batch][beams];
+ * beams <= 64; layers * batch <= 65,535. */
+psb_status psb_beam_reorder(const void* d_in, void* d_out, const int* d_parents, int layers, int batch, int beams, int heads, int tokens,
+                            int64_t token_bytes, const int* d_lengths, int device, void* stream);
+
 /* ---- synthetic data (bench and tests): counter-based generator, identical for any launch shape -------- */
 
 /* rows [row_begin, row_begin + n) of a Gaussian mixture in component-contiguous order:

@@ -107,6 +107,7 @@ EXPORTS = [
     "psb_sign_padded_dim", "psb_sign_rotation_scale", "psb_sign_rotate", "psb_sign_encode_database", "psb_sign_encode_queries", "psb_sign_search_candidates",
     "psb_kmeans_init", "psb_rotate_rows", "psb_stage_rotate_queries", "psb_scan_sample_words", "psb_stage_scan_sample", "psb_stage_scan_shared",
     "psb_ivf_layout_from_assignment", "psb_reorder_rows", "psb_coarse_host", "psb_coarse_search_static", "psb_knn_exact", "psb_kmeans_train", "psb_kmeans_assign", "psb_kmeans_accumulate", "psb_kmeans_update", "psb_residual_rows", "psb_pq_train", "psb_pq_encode", "psb_pq_encode_limited", "psb_gen_mixture_rows", "psb_gen_normal",
+    "psb_i8_encode_rows", "psb_i8_norm_rows", "psb_i8_matmul", "psb_i8_matmul_limited", "psb_beam_select", "psb_beam_reorder",
 ]
 
 _lib = None
@@ -828,6 +829,64 @@ def pq_encode_limited(d_data, n, dim, d_codebook, M, K, d_codes, items=-1, d_gav
     """Test hook of the time-out path of pq_encode's filter; see include/psb.h."""
     _check(lib().psb_pq_encode_limited(C.c_void_p(_p(d_data)), C.c_int64(n), dim, C.c_void_p(_p(d_codebook)), M, K, C.c_void_p(_p(d_codes)),
                                        C.c_int64(items), C.c_void_p(_p(d_gave_up)), device, _stream_ptr(stream)))
+
+
+# ---- rows of 8-bit codes, beams -------------------------------------------------------------------------
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+_TYPES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}
+
+
+def _type(tensor):
+    """PSB_TYPE_* of a tensor's elements."""
+    t = _TYPES.get(str(tensor.dtype))
+    if t is None:
+        raise InvalidArgument(1, "the elements are float32, float16 or bfloat16, not %s" % tensor.dtype)
+    return t
+
+
+def i8_encode_rows(d_rows, n, dim, d_codes, d_scales, row_stride=0, code_stride=0, device=0, stream=None):
+    """8-bit codes of n rows and a scale for each: row = codes * scale.  Strides in elements (0 = the rows lie side by side)."""
+    _check(lib().psb_i8_encode_rows(_vp(d_rows), _type(d_rows), C.c_int64(n), dim, C.c_int64(row_stride or dim), _vp(d_codes),
+                                    C.c_int64(code_stride or dim), _vp(d_scales), device, _stream_ptr(stream)))
+
+
+def i8_norm_rows(d_rows, n, dim, d_weight, eps, d_codes, d_scales, d_residual=None, d_sum=None, row_stride=0, residual_stride=0,
+                 sum_stride=0, code_stride=0, device=0, stream=None):
+    """8-bit codes of the root-mean-square norm of rows + residual; d_sum receives the sum, and may be d_rows or d_residual."""
+    kind = _type(d_rows)
+    for t in (d_weight, d_residual, d_sum):
+        if t is not None and _type(t) != kind:
+            raise InvalidArgument(1, "rows, weight, residual and sum are of one type")
+    _check(lib().psb_i8_norm_rows(_vp(d_rows), _vp(d_residual), _vp(d_weight), kind, C.c_int64(n), dim, C.c_int64(row_stride or dim),
+                                  C.c_int64(residual_stride or dim), C.c_float(eps), _vp(d_sum), C.c_int64(sum_stride or dim), _vp(d_codes),
+                                  C.c_int64(code_stride or dim), _vp(d_scales), device, _stream_ptr(stream)))
+
+
+def i8_matmul(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, x_stride=0, w_stride=0, out_stride=0, device=0, stream=None):
+    """out [m][n] = the products of m and n rows of k codes, with both sides' scales."""
+    _check(lib().psb_i8_matmul(_vp(d_x), C.c_int64(x_stride or k), _vp(d_x_scales), C.c_int64(m), _vp(d_w), C.c_int64(w_stride or k),
+                               _vp(d_w_scales), C.c_int64(n), k, _vp(d_out), _type(d_out), C.c_int64(out_stride or n), device,
+                               _stream_ptr(stream)))
+
+
+def i8_matmul_limited(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, tiles=-1, polls=1 << 22, x_stride=0, w_stride=0, out_stride=0,
+                      device=0, stream=None):
+    """Test hook of i8_matmul's time-out path; see include/psb.h."""
+    _check(lib().psb_i8_matmul_limited(_vp(d_x), C.c_int64(x_stride or k), _vp(d_x_scales), C.c_int64(m), _vp(d_w), C.c_int64(w_stride or k),
+                                       _vp(d_w_scales), C.c_int64(n), k, _vp(d_out), _type(d_out), C.c_int64(out_stride or n),
+                                       C.c_int64(tiles), polls, device, _stream_ptr(stream)))
+
+
+def beam_select(d_logits, d_scores, batch, beams, vocab, k, d_parents, d_tokens, d_totals, row_stride=0, device=0, stream=None):
+    """The k best continuations of every item over its beams and the vocabulary: parents and tokens [batch][k] int32, totals fp32."""
+    _check(lib().psb_beam_select(_vp(d_logits), _type(d_logits), C.c_int64(row_stride or vocab), _vp(d_scores), batch, beams, vocab, k,
+                                 _vp(d_parents), _vp(d_tokens), _vp(d_totals), device, _stream_ptr(stream)))
+
+
+def beam_reorder(d_in, d_out, d_parents, layers, batch, beams, heads, tokens, token_bytes, d_lengths=None, device=0, stream=None):
+    """States [layers][batch][beams][heads][tokens][token_bytes] in the order of the chosen parents; d_out may be d_in."""
+    _check(lib().psb_beam_reorder(_vp(d_in), _vp(d_out), _vp(d_parents), layers, batch, beams, heads, tokens, C.c_int64(token_bytes),
+                                  _vp(d_lengths), device, _stream_ptr(stream)))
 
 
 def gen_mixture_rows(d_centres, d_offsets, ncomp, dim, sigma, seed, row_begin, n, d_out, device=0, stream=None):

@@ -96,6 +96,16 @@ constexpr uint64_t KEY_MAX = ~0ull;
 psb_status kernel_shared(const void* kernel, size_t bytes);
 psb_status kernel_carveout_max(const void* kernel);
 
+// Makes `device` current for a call and the one that was current before again at its end; `sms`: its multiprocessors.
+struct DeviceScope {
+    int before = -1, sms = 0;
+    psb_status enter(int device);
+    DeviceScope() = default;
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+    ~DeviceScope();
+};
+
 #ifdef __CUDACC__
 // Asks for the maximum shared-memory carve-out for a kernel, whether or not it uses much shared memory.  An SM runs kernels of
 // one carve-out at a time; the scan, coarse and selection kernels need nearly all of it, so every kernel that may run beside

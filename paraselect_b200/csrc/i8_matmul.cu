@@ -1,0 +1,391 @@
+// Products of rows of 8-bit codes with a scale for each row on both sides:
+//   out[i][j] = x_scale[i] w_scale[j] sum_k x[i][k] w[j][k].
+// The sum is exact (int32 on the tensor cores, tcgen05 kind::i8), the scaling is three fp32 roundings, the output's type one more.
+//
+// The rows of w (channels, stored rows) take the tensor cores' M side, 128 to a block, and the rows of x (tokens, queries) the N side, up to
+// 256: a thread of the epilogue then holds one channel for all tokens, a warp 32 neighbouring channels, and its stores of a token's outputs
+// lie side by side without a pass through shared memory.  One token is the same kernel with 16 columns, bound by the reading of w.
+//
+// k runs through shared memory in slabs of 128 codes (one 128-byte swizzle row), loaded by TMA into a ring; codes behind the end of a row and
+// rows behind the last are the TMA's zeros.  Few tiles are split along k over a cluster of up to 8 blocks, which hold their partial sums in
+// shared memory and add them there: integers, so the order does not matter.
+//
+// Waits on the device are bounded.  A block whose wait gave up waits for what it has issued, frees its tensor memory and forms its outputs
+// with dp4a instead, so that the results are the same.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "tc_ptx.cuh"
+
+namespace psb {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kSlab = 128;                 // codes of a row in a slab: one swizzle row
+constexpr int kChannels = 128;             // rows of w a block
+constexpr int kMaxTokens = 256;            // rows of x a tile
+constexpr int kThreads = 192;              // four epilogue warps, one that loads, one that issues products
+constexpr int kMaxStages = 12;
+constexpr int kRing = 200 * 1024;
+constexpr int kWaitPolls = 1 << 22;
+
+struct MatmulArgs {
+    const signed char* x;
+    const signed char* w;
+    const float* x_scales;
+    const float* w_scales;
+    void* out;
+    long long x_stride, w_stride, out_stride;
+    int m, n, k;                           // tokens, channels, codes a row
+    int tokens;                            // rows of x a tile: a multiple of 16
+    int stages, slabs;
+    int channel_tiles, tiles;
+    long long issued;                      // tiles that get their products (all but in tests)
+    int polls;
+};
+
+// kind::i8 instruction descriptor: D int32, A and B signed, both K-major.
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+template <typename T> __device__ __forceinline__ T rounded(float v);
+template <> __device__ __forceinline__ float rounded<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__host__ __device__ inline int tmem_columns(int tokens, int buffers) {
+    int c = 32;
+    while (c < tokens * buffers) c <<= 1;
+    return c;
+}
+
+// The dot product of two rows of codes, four at a time (rows begin at multiples of 16 bytes).
+__device__ int dot_codes(const signed char* a, const signed char* b, int k) {
+    int s = 0, i = 0;
+    for (; i + 4 <= k; i += 4) s = __dp4a(*reinterpret_cast<const int*>(a + i), *reinterpret_cast<const int*>(b + i), s);
+    for (; i < k; ++i) s += (int)a[i] * (int)b[i];
+    return s;
+}
+
+// SPLIT: the blocks of a cluster share a tile, each with its share of the slabs.  Otherwise a block takes every gridDim.x-th tile, its
+// accumulators in two buffers, so that the epilogue of one tile lies beside the products of the next.
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MatmulArgs a) {
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], ready[2], drained[2], last;
+    __shared__ uint32_t tmem_at;
+    __shared__ int gave_up;
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int parts = SPLIT ? (int)cg::this_cluster().num_blocks() : 1;
+    const int part = SPLIT ? (int)cg::this_cluster().block_rank() : 0;
+    const int first = SPLIT ? (int)blockIdx.x / parts : (int)blockIdx.x;
+    const int step = SPLIT ? a.tiles : (int)gridDim.x;         // a split tile is its cluster's only one
+    const int slab0 = a.slabs * part / parts, slab1 = a.slabs * (part + 1) / parts;
+    const int stage_bytes = (kChannels + a.tokens) * kSlab;
+    constexpr int kBuffers = SPLIT ? 1 : 2;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < a.stages; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&ready[i], 1); tc::mbar_init(&drained[i], 4); }
+        tc::mbar_init(&last, 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
+        }
+    } else if (warp == 5) {
+        tc::tmem_alloc(&tmem_at, tmem_columns(a.tokens, kBuffers));
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp == 4) {
+        if (tc::elect_one()) {
+            int at = 0;
+            bool ok = true;
+            for (int tile = first; ok && tile < a.tiles; tile += step) {
+                const int c0 = tile % a.channel_tiles * kChannels, t0 = tile / a.channel_tiles * a.tokens;
+                for (int slab = slab0; slab < slab1; ++slab, ++at) {
+                    const int st = at % a.stages;
+                    if (at >= a.stages && !tc::mbar_wait(&empty[st], (at / a.stages - 1) & 1, a.polls)) { ok = false; break; }
+                    tc::mbar_expect_tx(&full[st], stage_bytes);
+                    unsigned char* to = ring + st * stage_bytes;
+                    tc::tma_load_2d(to, &map_w, slab * kSlab, c0, &full[st]);
+                    tc::tma_load_2d(to + kChannels * kSlab, &map_x, slab * kSlab, t0, &full[st]);
+                }
+            }
+            if (!ok) {   // the loads under way land before the block ends
+                gave_up = 1;
+                for (int i = max(0, at - a.stages); i < at; ++i) tc::mbar_wait(&full[i % a.stages], (i / a.stages) & 1, a.polls);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        if (tc::elect_one()) {
+            const uint32_t idesc = idesc_i8(kChannels, a.tokens);
+            int at = 0, count = 0;
+            bool ok = true;
+            for (int tile = first; ok && tile < a.tiles; tile += step, ++count) {
+                const int buf = count % kBuffers;
+                if (count >= kBuffers && !tc::mbar_wait(&drained[buf], (count / kBuffers - 1) & 1, a.polls)) { ok = false; break; }
+                if (tile >= a.issued) { ok = false; break; }
+                tc::tc_fence_after();
+                for (int slab = slab0; slab < slab1; ++slab, ++at) {
+                    const int st = at % a.stages;
+                    if (!tc::mbar_wait(&full[st], (at / a.stages) & 1, a.polls)) { ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t w_at = tc::smem_u32(ring + st * stage_bytes);
+                    const uint64_t dw = tc::make_sw128_desc(w_at), dx = tc::make_sw128_desc(w_at + kChannels * kSlab);
+#pragma unroll
+                    for (int q = 0; q < kSlab / 32; ++q) umma_i8(tmem + buf * a.tokens, dw + 2 * q, dx + 2 * q, idesc, slab > slab0 || q > 0);
+                    tc::umma_commit(&empty[st]);
+                }
+                if (ok) tc::umma_commit(&ready[buf]);
+            }
+            if (!ok) {   // the products under way end before the tensor memory is freed
+                gave_up = 1;
+                tc::umma_commit(&last);
+                tc::mbar_wait(&last, 0, a.polls);
+            }
+        }
+        __syncwarp();
+    } else {
+        int count = 0;
+        for (int tile = first; tile < a.tiles; tile += step, ++count) {
+            const int buf = count % kBuffers;
+            const int c0 = tile % a.channel_tiles * kChannels, t0 = tile / a.channel_tiles * a.tokens;
+            if (!tc::mbar_wait(&ready[buf], (count / kBuffers) & 1, a.polls)) { gave_up = 1; break; }
+            __syncwarp();
+            tc::tc_fence_after();
+            const uint32_t from = tmem + buf * a.tokens + ((uint32_t)(warp * 32) << 16);
+            const int c = c0 + warp * 32 + lane;
+            if constexpr (SPLIT) {   // all products have ended: the ring is free for the partial sums, [token][channel]
+                int* partial = reinterpret_cast<int*>(ring);
+                for (int t = 0; t < a.tokens; t += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(from + t, v);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) partial[(t + i) * kChannels + warp * 32 + lane] = (int)v[i];
+                }
+            } else {
+                const float ws = c < a.n ? __ldg(a.w_scales + c) : 0.f;
+                T* out = static_cast<T*>(a.out) + c;
+                for (int t = 0; t < a.tokens && t0 + t < a.m; t += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(from + t, v);
+                    const float xs = t0 + t + (lane & 15) < a.m ? __ldg(a.x_scales + t0 + t + (lane & 15)) : 0.f;
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float by = __shfl_sync(0xffffffffu, xs, i);
+                        if (c < a.n && t0 + t + i < a.m) out[(long long)(t0 + t + i) * a.out_stride] = rounded<T>((float)(int)v[i] * by * ws);
+                    }
+                }
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&drained[buf])) : "memory");
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 5) tc::tmem_dealloc(tmem, tmem_columns(a.tokens, kBuffers));
+
+    if constexpr (SPLIT) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        int lost = 0;
+        for (int p = 0; p < parts; ++p) lost |= *cluster.map_shared_rank(&gave_up, p);
+        const int c0 = first % a.channel_tiles * kChannels, t0 = first / a.channel_tiles * a.tokens;
+        const int* partial = reinterpret_cast<const int*>(ring);
+        // four channels a thread: 32 threads a token
+        const int c4 = (threadIdx.x & 31) * 4;
+        for (int t = part * 6 + warp; t < a.tokens && t0 + t < a.m; t += 6 * parts) {
+            int s[4] = {0, 0, 0, 0};
+            if (!lost) {
+                for (int p = 0; p < parts; ++p) {
+                    const int4 v = *reinterpret_cast<const int4*>(cluster.map_shared_rank(partial, p) + t * kChannels + c4);
+                    s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+                }
+            } else {
+                for (int e = 0; e < 4; ++e)
+                    if (c0 + c4 + e < a.n) s[e] = dot_codes(a.x + (t0 + t) * a.x_stride, a.w + (c0 + c4 + e) * a.w_stride, a.k);
+            }
+            const float by = __ldg(a.x_scales + t0 + t);
+            T* out = static_cast<T*>(a.out) + (long long)(t0 + t) * a.out_stride + c0 + c4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c0 + c4 + e < a.n) out[e] = rounded<T>((float)s[e] * by * __ldg(a.w_scales + c0 + c4 + e));
+        }
+        cluster.sync();   // no block ends while another reads its sums
+    } else if (gave_up) {
+        for (int tile = first; tile < a.tiles; tile += step) {
+            const int c0 = tile % a.channel_tiles * kChannels, t0 = tile / a.channel_tiles * a.tokens;
+            for (int i = threadIdx.x; i < kChannels * a.tokens; i += kThreads) {
+                const int c = c0 + i % kChannels, t = t0 + i / kChannels;
+                if (c < a.n && t < a.m)
+                    static_cast<T*>(a.out)[(long long)t * a.out_stride + c] =
+                        rounded<T>((float)dot_codes(a.x + t * a.x_stride, a.w + c * a.w_stride, a.k) * __ldg(a.x_scales + t) * __ldg(a.w_scales + c));
+            }
+        }
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+psb_status encode_fn(EncodeTiledFn* out) {
+    static std::atomic<EncodeTiledFn> known{nullptr};
+    EncodeTiledFn fn = known.load(std::memory_order_acquire);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        PSB_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found));
+        if (!p || found != cudaDriverEntryPointSuccess) return fail(PSB_CUDA_ERROR, "cuTensorMapEncodeTiled is not available");
+        fn = reinterpret_cast<EncodeTiledFn>(p);
+        known.store(fn, std::memory_order_release);
+    }
+    *out = fn;
+    return PSB_OK;
+}
+
+// Rows of k codes, `box_rows` of them and a slab of codes at a time.
+psb_status codes_map(CUtensorMap* map, const void* base, int64_t rows, int k, int64_t stride, int box_rows) {
+    EncodeTiledFn fn;
+    PSB_TRY(encode_fn(&fn));
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)kSlab, (cuuint32_t)box_rows};
+    const cuuint32_t every[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, every, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(PSB_CUDA_ERROR, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+    return PSB_OK;
+}
+
+template <typename T>
+psb_status run(MatmulArgs a, int sms, cudaStream_t s) {
+    // tiles of tokens of even size, each a multiple of 16
+    const int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
+    a.tokens = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    a.channel_tiles = (a.n + kChannels - 1) / kChannels;
+    const long long tiles = (long long)token_tiles * a.channel_tiles;
+    if (tiles > 0x7fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^31 - 1 tiles of 128 x 256 outputs");
+    a.tiles = (int)tiles;
+    a.slabs = (a.k + kSlab - 1) / kSlab;
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= sms && a.slabs >= parts * 4) parts *= 2;
+    const int stage_bytes = (kChannels + a.tokens) * kSlab;
+    a.stages = std::min(kMaxStages, kRing / stage_bytes);
+    const size_t smem = 1024 + std::max((size_t)a.stages * stage_bytes, parts > 1 ? (size_t)a.tokens * kChannels * 4 : 0);
+    CUtensorMap map_w, map_x;
+    PSB_TRY(codes_map(&map_w, a.w, a.n, a.k, a.w_stride, kChannels));
+    PSB_TRY(codes_map(&map_x, a.x, a.m, a.k, a.x_stride, a.tokens));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr = {};
+    if (parts > 1) {
+        PSB_TRY(kernel_shared(reinterpret_cast<const void*>(k_i8_matmul<T, true>), smem));
+        cfg.gridDim = dim3((unsigned)(a.tiles * parts));
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr; cfg.numAttrs = 1;
+        PSB_CUDA(cudaLaunchKernelEx(&cfg, k_i8_matmul<T, true>, map_w, map_x, a));
+    } else {
+        PSB_TRY(kernel_shared(reinterpret_cast<const void*>(k_i8_matmul<T, false>), smem));
+        cfg.gridDim = dim3((unsigned)std::min<long long>(tiles, sms));
+        PSB_CUDA(cudaLaunchKernelEx(&cfg, k_i8_matmul<T, false>, map_w, map_x, a));
+    }
+    count_launch();
+    return PSB_OK;
+}
+
+constexpr int kMaxDepth = 131071;   // 128 * 128 * k stays below 2^31
+
+psb_status matmul(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride, const float* d_w_scales, int64_t n, int k,
+                  void* d_out, int out_type, int64_t out_stride, long long issued, int polls, int device, void* stream) {
+    if (m < 0 || n < 0 || k <= 0 || out_type < PSB_TYPE_F32 || out_type > PSB_TYPE_BF16) return fail(PSB_INVALID_ARGUMENT, "product of codes: a size below its least or an unknown type");
+    if (k > kMaxDepth || m > 0x7fffff00 || n > 0x7fffff00) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: at most 131,071 codes a row and 2^31 - 256 rows");
+    if (x_stride < k || w_stride < k || out_stride < n) return fail(PSB_INVALID_ARGUMENT, "product of codes: a stride is less than a row");
+    if (m == 0 || n == 0) return PSB_OK;
+    if (!d_x || !d_w || !d_x_scales || !d_w_scales || !d_out) return fail(PSB_INVALID_ARGUMENT, "product of codes: a null pointer");
+    auto at = [](const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; };
+    if (!at(d_x, 16) || !at(d_w, 16) || x_stride % 16 || w_stride % 16)
+        return fail(PSB_INVALID_ARGUMENT, "product of codes: rows of codes begin at multiples of 16 bytes, their strides are multiples of 16");
+    if (x_stride >= (1ll << 40) || w_stride >= (1ll << 40)) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: a stride of 2^40 bytes or more");
+    const size_t e = out_type == PSB_TYPE_F32 ? 4 : 2;
+    if (!at(d_out, e) || !at(d_x_scales, 4) || !at(d_w_scales, 4)) return fail(PSB_INVALID_ARGUMENT, "product of codes: a pointer is not aligned to its elements");
+    const uintptr_t o0 = reinterpret_cast<uintptr_t>(d_out), o1 = o0 + ((uintptr_t)(m - 1) * out_stride + n) * e;
+    auto apart = [&](const void* p, int64_t rows, int64_t stride, int64_t width) {
+        const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+        return b >= o1 || b + (uintptr_t)(rows - 1) * stride + width <= o0;
+    };
+    if (!apart(d_x, m, x_stride, k) || !apart(d_w, n, w_stride, k) || !apart(d_x_scales, m, 4, 4) || !apart(d_w_scales, n, 4, 4))
+        return fail(PSB_INVALID_ARGUMENT, "product of codes: the output lies over an input");
+    DeviceScope on;
+    PSB_TRY(on.enter(device));
+    MatmulArgs a{};
+    a.x = reinterpret_cast<const signed char*>(d_x); a.w = reinterpret_cast<const signed char*>(d_w);
+    a.x_scales = d_x_scales; a.w_scales = d_w_scales; a.out = d_out;
+    a.x_stride = x_stride; a.w_stride = w_stride; a.out_stride = out_stride;
+    a.m = (int)m; a.n = (int)n; a.k = k; a.issued = issued; a.polls = polls;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (out_type) {
+        case PSB_TYPE_F32: return run<float>(a, on.sms, s);
+        case PSB_TYPE_F16: return run<__half>(a, on.sms, s);
+        default: return run<__nv_bfloat16>(a, on.sms, s);
+    }
+}
+
+}  // namespace
+}  // namespace psb
+
+using namespace psb;
+
+extern "C" {
+
+psb_status psb_i8_matmul(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride, const float* d_w_scales, int64_t n,
+                         int k, void* d_out, int out_type, int64_t out_stride, int device, void* stream) {
+    return matmul(d_x, x_stride, d_x_scales, m, d_w, w_stride, d_w_scales, n, k, d_out, out_type, out_stride, 0x7fffffffffffffffll, kWaitPolls, device, stream);
+}
+
+psb_status psb_i8_matmul_limited(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride, const float* d_w_scales,
+                                 int64_t n, int k, void* d_out, int out_type, int64_t out_stride, int64_t tiles, int polls, int device, void* stream) {
+    if (polls <= 0) return fail(PSB_INVALID_ARGUMENT, "product of codes: a wait without polls");
+    return matmul(d_x, x_stride, d_x_scales, m, d_w, w_stride, d_w_scales, n, k, d_out, out_type, out_stride, tiles < 0 ? 0x7fffffffffffffffll : tiles, polls, device,
+                  stream);
+}
+
+}  // extern "C"

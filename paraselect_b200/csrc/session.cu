@@ -175,6 +175,18 @@ psb_status check_device(int device, int* sm_count = nullptr) {
     return PSB_OK;
 }
 
+}  // namespace
+psb_status DeviceScope::enter(int device) {
+    int now = -1;
+    if (cudaGetDevice(&now) != cudaSuccess) { cudaGetLastError(); now = -1; }   // check_device says what is wrong
+    PSB_TRY(check_device(device, &sms));
+    if (now != device) before = now;
+    return PSB_OK;
+}
+DeviceScope::~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
+
+namespace {
+
 // Work memory of the operators that allocate, run and free within one call (training, one-shot searches): from a memory pool of
 // the library per device, stream-ordered, so that a call pays neither cudaMalloc nor the device synchronisation of cudaFree (about
 // a third of a small training call).  The pool keeps at most kPoolKeep bytes between calls; what is above goes back to the device at
