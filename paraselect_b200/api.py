@@ -833,21 +833,47 @@ def pq_encode_limited(d_data, n, dim, d_codebook, M, K, d_codes, items=-1, d_gav
 
 # ---- rows of 8-bit codes, beams -------------------------------------------------------------------------
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
-_TYPES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}
+_TYPE_NAMES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}
+_types = {}   # a tensor library's type object -> PSB_TYPE_*
 
 
 def _type(tensor):
     """PSB_TYPE_* of a tensor's elements."""
-    t = _TYPES.get(str(tensor.dtype))
+    t = _types.get(tensor.dtype)
     if t is None:
+        t = _types[tensor.dtype] = _TYPE_NAMES.get(str(tensor.dtype), -1)
+    if t < 0:
         raise InvalidArgument(1, "the elements are float32, float16 or bfloat16, not %s" % tensor.dtype)
     return t
 
 
+_V, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
+_OPERATOR_ARGS = {
+    "psb_i8_encode_rows": [_V, _I, _L, _I, _L, _V, _L, _V, _I, _V],
+    "psb_i8_norm_rows": [_V, _V, _V, _I, _L, _I, _L, _L, _F, _V, _L, _V, _L, _V, _I, _V],
+    "psb_i8_matmul": [_V, _L, _V, _L, _V, _L, _V, _L, _I, _V, _I, _L, _I, _V],
+    "psb_i8_matmul_limited": [_V, _L, _V, _L, _V, _L, _V, _L, _I, _V, _I, _L, _L, _I, _I, _V],
+    "psb_beam_select": [_V, _I, _L, _V, _I, _I, _I, _I, _V, _V, _V, _I, _V],
+    "psb_beam_reorder": [_V, _V, _V, _I, _I, _I, _I, _I, _L, _V, _I, _V],
+}
+_operators = {}
+
+
+def _call(name, *args):
+    """A call with declared argument types: these operators take microseconds, and building a ctypes object for each argument took as long."""
+    fn = _operators.get(name)
+    if fn is None or fn[0] is not _lib:
+        f = getattr(lib(), name)
+        f.argtypes = _OPERATOR_ARGS[name]
+        fn = _operators[name] = (_lib, f)
+    status = fn[1](*args)
+    if status != PSB_OK:
+        _check(status)
+
+
 def i8_encode_rows(d_rows, n, dim, d_codes, d_scales, row_stride=0, code_stride=0, device=0, stream=None):
     """8-bit codes of n rows and a scale for each: row = codes * scale.  Strides in elements (0 = the rows lie side by side)."""
-    _check(lib().psb_i8_encode_rows(_vp(d_rows), _type(d_rows), C.c_int64(n), dim, C.c_int64(row_stride or dim), _vp(d_codes),
-                                    C.c_int64(code_stride or dim), _vp(d_scales), device, _stream_ptr(stream)))
+    _call("psb_i8_encode_rows", _p(d_rows), _type(d_rows), n, dim, row_stride or dim, _p(d_codes), code_stride or dim, _p(d_scales), device, stream)
 
 
 def i8_norm_rows(d_rows, n, dim, d_weight, eps, d_codes, d_scales, d_residual=None, d_sum=None, row_stride=0, residual_stride=0,
@@ -857,36 +883,32 @@ def i8_norm_rows(d_rows, n, dim, d_weight, eps, d_codes, d_scales, d_residual=No
     for t in (d_weight, d_residual, d_sum):
         if t is not None and _type(t) != kind:
             raise InvalidArgument(1, "rows, weight, residual and sum are of one type")
-    _check(lib().psb_i8_norm_rows(_vp(d_rows), _vp(d_residual), _vp(d_weight), kind, C.c_int64(n), dim, C.c_int64(row_stride or dim),
-                                  C.c_int64(residual_stride or dim), C.c_float(eps), _vp(d_sum), C.c_int64(sum_stride or dim), _vp(d_codes),
-                                  C.c_int64(code_stride or dim), _vp(d_scales), device, _stream_ptr(stream)))
+    _call("psb_i8_norm_rows", _p(d_rows), _p(d_residual), _p(d_weight), kind, n, dim, row_stride or dim, residual_stride or dim, eps,
+          _p(d_sum), sum_stride or dim, _p(d_codes), code_stride or dim, _p(d_scales), device, stream)
 
 
 def i8_matmul(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, x_stride=0, w_stride=0, out_stride=0, device=0, stream=None):
     """out [m][n] = the products of m and n rows of k codes, with both sides' scales."""
-    _check(lib().psb_i8_matmul(_vp(d_x), C.c_int64(x_stride or k), _vp(d_x_scales), C.c_int64(m), _vp(d_w), C.c_int64(w_stride or k),
-                               _vp(d_w_scales), C.c_int64(n), k, _vp(d_out), _type(d_out), C.c_int64(out_stride or n), device,
-                               _stream_ptr(stream)))
+    _call("psb_i8_matmul", _p(d_x), x_stride or k, _p(d_x_scales), m, _p(d_w), w_stride or k, _p(d_w_scales), n, k, _p(d_out), _type(d_out),
+          out_stride or n, device, stream)
 
 
 def i8_matmul_limited(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, tiles=-1, polls=1 << 22, x_stride=0, w_stride=0, out_stride=0,
                       device=0, stream=None):
     """Test hook of i8_matmul's time-out path; see include/psb.h."""
-    _check(lib().psb_i8_matmul_limited(_vp(d_x), C.c_int64(x_stride or k), _vp(d_x_scales), C.c_int64(m), _vp(d_w), C.c_int64(w_stride or k),
-                                       _vp(d_w_scales), C.c_int64(n), k, _vp(d_out), _type(d_out), C.c_int64(out_stride or n),
-                                       C.c_int64(tiles), polls, device, _stream_ptr(stream)))
+    _call("psb_i8_matmul_limited", _p(d_x), x_stride or k, _p(d_x_scales), m, _p(d_w), w_stride or k, _p(d_w_scales), n, k, _p(d_out),
+          _type(d_out), out_stride or n, tiles, polls, device, stream)
 
 
 def beam_select(d_logits, d_scores, batch, beams, vocab, k, d_parents, d_tokens, d_totals, row_stride=0, device=0, stream=None):
     """The k best continuations of every item over its beams and the vocabulary: parents and tokens [batch][k] int32, totals fp32."""
-    _check(lib().psb_beam_select(_vp(d_logits), _type(d_logits), C.c_int64(row_stride or vocab), _vp(d_scores), batch, beams, vocab, k,
-                                 _vp(d_parents), _vp(d_tokens), _vp(d_totals), device, _stream_ptr(stream)))
+    _call("psb_beam_select", _p(d_logits), _type(d_logits), row_stride or vocab, _p(d_scores), batch, beams, vocab, k, _p(d_parents),
+          _p(d_tokens), _p(d_totals), device, stream)
 
 
 def beam_reorder(d_in, d_out, d_parents, layers, batch, beams, heads, tokens, token_bytes, d_lengths=None, device=0, stream=None):
     """States [layers][batch][beams][heads][tokens][token_bytes] in the order of the chosen parents; d_out may be d_in."""
-    _check(lib().psb_beam_reorder(_vp(d_in), _vp(d_out), _vp(d_parents), layers, batch, beams, heads, tokens, C.c_int64(token_bytes),
-                                  _vp(d_lengths), device, _stream_ptr(stream)))
+    _call("psb_beam_reorder", _p(d_in), _p(d_out), _p(d_parents), layers, batch, beams, heads, tokens, token_bytes, _p(d_lengths), device, stream)
 
 
 def gen_mixture_rows(d_centres, d_offsets, ncomp, dim, sigma, seed, row_begin, n, d_out, device=0, stream=None):

@@ -6,7 +6,8 @@
 // maximum and a sum.  From those every block has each beam's log-sum, and a bound: of all shares' maxima, as totals, the k-th largest - at
 // least k totals reach it.  Only shares whose maximum reaches the bound, hardly more than k of them, are looked through again for the totals
 // that do; the few found are ranked by the cluster's first block.  Sums are held in fp32 within a lane (some hundred terms) and in 64 bits
-// beyond, totals are compared in 64 bits.
+// beyond, totals are compared in 64 bits.  The warps of a cluster are dealt out to the beams, so that a warp of a small call waits for one
+// round of loads and reduces once.
 //
 // What a lane reads and adds depends on the tokens' numbers alone, not on a row's address, so that equal rows have equal totals.
 #include <cooperative_groups.h>
@@ -14,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -30,7 +32,7 @@ constexpr int kLine = 256;              // tokens that a warp reads at once: 8 n
 constexpr int kMaxBeams = 64;
 constexpr int kMaxChosen = 64;
 constexpr int kMaxCluster = 16;
-constexpr int kMaxGroups = 512;         // shares are joined to at most so many for the bound
+constexpr int kMaxShares = kMaxCluster * kWarps;
 constexpr int kFoundCap = 2048;
 
 struct SelectArgs {
@@ -41,13 +43,10 @@ struct SelectArgs {
     float* totals;
     long long row_stride;
     int beams, vocab, k, lines;
-    int join;                           // shares of a beam joined for the bound
+    int per_beam;                       // warps that share a beam's row; share s is part s % per_beam of beam s / per_beam, and its warp's (s / warps)-th
+    int join;                           // shares joined for the bound
     bool wide;                          // rows begin at multiples of 16 bytes
 };
-
-__device__ __forceinline__ float value(float v) { return v; }
-__device__ __forceinline__ float value(__half v) { return __half2float(v); }
-__device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // 2^v to 2 units in the last place; results below 2^-126 are zero, which a sum of one or more does not notice.
 __device__ __forceinline__ float exp2_of(float v) {
@@ -57,20 +56,64 @@ __device__ __forceinline__ float exp2_of(float v) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Eight neighbouring tokens' logits; -inf behind the vocabulary's end.
-template <typename T>
-__device__ __forceinline__ void read8(const T* row, int at, int vocab, bool wide, float (&x)[8]) {
-    if (wide && at + 8 <= vocab) {
-        alignas(16) T v[8];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(row + at) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = value(v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = at + i < vocab ? value(row[at + i]) : -INFINITY;
-    }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
+__device__ __forceinline__ float2 halves(unsigned long long p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// The largest of a warp's values, for all its lanes.
+__device__ __forceinline__ float warp_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Eight neighbouring tokens' logits as they lie in memory; -inf behind the vocabulary's end.
+template <typename T> struct Raw8 {
+    static constexpr int kWords = 2 * sizeof(T);
+    unsigned word[kWords];
+    __device__ __forceinline__ void read(const T* row, int at, int vocab, bool wide) {
+        if (wide && at + 8 <= vocab) {
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + at) + i);
+                word[4 * i] = v.x; word[4 * i + 1] = v.y; word[4 * i + 2] = v.z; word[4 * i + 3] = v.w;
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) word[i] = at + i < vocab ? __float_as_uint(__ldg(reinterpret_cast<const float*>(row) + at + i)) : 0xff800000u;
+            else {
+                constexpr unsigned kLow = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+                const unsigned short* u = reinterpret_cast<const unsigned short*>(row);
+                const unsigned lo = at + 2 * i < vocab ? __ldg(u + at + 2 * i) : kLow, hi = at + 2 * i + 1 < vocab ? __ldg(u + at + 2 * i + 1) : kLow;
+                word[i] = lo | hi << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ float2 two(int i) const {   // logits 2 i and 2 i + 1
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(word[2 * i]), __uint_as_float(word[2 * i + 1]));
+        else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&word[i]));
+        else return make_float2(__uint_as_float(word[i] << 16), __uint_as_float(word[i] & 0xffff0000u));
+    }
+};
 
 // Totals as integers of the same order (a total is never NaN).
 __device__ __forceinline__ unsigned long long ordered(double v) {
@@ -82,22 +125,23 @@ __device__ __forceinline__ double from_ordered(unsigned long long o) { return __
 struct Found { unsigned long long total; unsigned at; unsigned pad; };   // at = beam * vocab + token
 __device__ __forceinline__ bool before(const Found& a, const Found& b) { return a.total > b.total || (a.total == b.total && a.at < b.at); }
 
+// The largest logit, and the sum of exp2((x - base) kLog2e) over the share's tokens.  base = (top kLog2e) / kLog2e with the product rounded to fp32,
+// so that an exponent takes one fused operation and what the rounding changed is known; where that product leaves fp32, the logit itself.
 struct Share { float top; double sum; };
+__device__ __forceinline__ bool huge(float top) { return fabsf(top) > 1e38f; }
+__device__ __forceinline__ double base_of(float top) { return huge(top) ? (double)top : (double)(top * kLog2e) / (double)kLog2e; }
 
 struct SelectShared {
-    Share shares[kMaxBeams][kWarps];
+    Share shares[kMaxShares];                        // of the whole item, written by their warps in every block
+    float parts[kMaxBeams / kWarps][kWarps][32];     // the largest logits of 32 parts of this block's shares
     Found found[kFoundCap];
     int count;
-    // of the whole item, the same in every block
-    float group_top[kMaxGroups];
-    double group_sum[kMaxGroups];
-    float reach[kMaxGroups];
-    float top[kMaxBeams];
-    double log_sum[kMaxBeams], score[kMaxBeams];
-    bool open[kMaxBeams];               // the beam offers continuations
+    float reach[kMaxShares];
+    double base[kMaxBeams], log_sum[kMaxBeams], score[kMaxBeams];
+    bool open[kMaxBeams];                            // the beam offers continuations
     float bound;
-    Found all[kMaxCluster * kMaxChosen];
-    int counts[kMaxCluster + 1];
+    Found all[kMaxCluster][kMaxChosen];              // in the cluster's first block: what every block found
+    int counts[kMaxCluster];
 };
 
 // The found ones beyond the k best go; the k best stay in no order.  For all threads of the block.
@@ -125,97 +169,117 @@ __device__ void keep_best(SelectShared& s, int k) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_beam_select(SelectArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
     SelectShared& s = *reinterpret_cast<SelectShared*>(raw);
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const long long item = blockIdx.x / blocks;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int warps = blocks * kWarps, me = rank * kWarps + warp;
+    const int warps = blocks * kWarps, me = rank * kWarps + warp, shares = a.per_beam * a.beams;
     const T* rows = static_cast<const T*>(a.logits) + item * a.beams * a.row_stride;
-    if (threadIdx.x == 0) s.count = 0;
+    if (threadIdx.x == 0) { s.count = 0; s.bound = -INFINITY; }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // waited for before the first write to another block
 
-    // The warps take the lines of all beams in turn, so that short rows spread as well: line l of beam b goes to warp (b lines + l) % warps.
-    auto first_line = [&](int b) { const int r = (int)((me - (long long)b * a.lines) % warps); return r < 0 ? r + warps : r; };
-    for (int b = 0; b < a.beams; ++b) {
-        const T* row = rows + b * a.row_stride;
-        float top = -INFINITY, sum = 0.f;
-        for (int l0 = first_line(b); l0 < a.lines; l0 += 4 * warps) {
-            float x[4][8];
+    // A share's lines are per_beam apart, kLines of them at a time, read ahead by as many.
+    constexpr int kLines = 16 / sizeof(T) / 2;
+    const int steps = (a.lines + kLines * a.per_beam - 1) / (kLines * a.per_beam);
+    int shift = 0;   // 32 parts at most, of 2^shift steps
+    while ((steps - 1) >> shift >= 32) ++shift;
+    auto read = [&](const T* row, int line, Raw8<T> (&x)[kLines]) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int l = l0 + u * warps;
-                if (l < a.lines) read8(row, l * kLine + lane * 8, a.vocab, a.wide, x[u]);
-                else
+        for (int u = 0; u < kLines; ++u)
+            if (line + u * a.per_beam < a.lines) x[u].read(row, (line + u * a.per_beam) * kLine + lane * 8, a.vocab, a.wide);
+    };
+    for (int share = me, turn = 0; share < shares; share += warps, ++turn) {
+        const T* row = rows + share / a.per_beam * a.row_stride;
+        float top = -INFINITY, at = 0.f, part = -INFINITY;
+        unsigned long long sums = 0;   // two sums of zero
+        Raw8<T> x[kLines], next[kLines];
+        int line = share % a.per_beam;
+        read(row, line, x);
+        for (int step = 0; step < steps; ++step, line += kLines * a.per_beam) {
+            if (step + 1 < steps) read(row, line + kLines * a.per_beam, next);
+            float t = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[u][i] = -INFINITY;
+            for (int u = 0; u < kLines; ++u)
+                if (line + u * a.per_beam < a.lines)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { const float2 v = x[u].two(i); t = fmaxf(t, fmaxf(v.x, v.y)); }
+            const float most = warp_max(t);
+            if (lane == step >> shift) part = fmaxf(part, most);
+            if (most > top) {   // the same for all lanes: the sums come down to the new base
+                const float to = most * kLog2e;
+                const float by = top == -INFINITY ? 0.f : huge(top) || huge(most) ? exp2_of((top - most) * kLog2e) : exp2_of(at - to);
+                const float2 v = halves(sums);
+                sums = pair(v.x * by, v.y * by);
+                top = most; at = to;
             }
-            float t = top;
+            if (huge(top) && top != -INFINITY) {
+#pragma unroll 1
+                for (int u = 0; u < kLines; ++u)
+                    if (line + u * a.per_beam < a.lines) {
+                        Raw8<T> y;
+                        y.read(row, (line + u * a.per_beam) * kLine + lane * 8, a.vocab, a.wide);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+                        for (int i = 0; i < 4; ++i) { const float2 v = y.two(i); sums = add2(sums, pair(exp2_of((v.x - top) * kLog2e), exp2_of((v.y - top) * kLog2e))); }
+                    }
+            } else {
+                const unsigned long long scale = pair(kLog2e, kLog2e), less = pair(-at, -at);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t = fmaxf(t, x[u][i]);
-            // without a finite maximum only infinities or NaN were seen, which the sum has to show
-            const float base = t == -INFINITY ? 0.f : t;
-            sum *= exp2_of((top - base) * kLog2e);
-            top = t;
+                for (int u = 0; u < kLines; ++u)
+                    if (line + u * a.per_beam < a.lines)
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 v = x[u].two(i), e = halves(fma2(pair(v.x, v.y), scale, less));
+                            sums = add2(sums, pair(exp2_of(e.x), exp2_of(e.y)));
+                        }
+            }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += exp2_of((x[u][i] - base) * kLog2e);
+            for (int u = 0; u < kLines; ++u) x[u] = next[u];
         }
-        // lanes to a share; a lane without a finite maximum has a sum of zero or NaN
-        float all = top;
+        // without a finite maximum the sum is zero or, with a NaN or an infinity among the logits, NaN
+        const float2 v = halves(sums);
+        double sum = (double)v.x + (double)v.y;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-        double part = top == -INFINITY ? (double)sum : (double)sum * (double)exp2_of((top - all) * kLog2e);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-        if (lane == 0) s.shares[b][warp] = Share{all, part};
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        s.parts[turn][warp][lane] = part;
+        if (turn == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (lane < blocks) *cluster.map_shared_rank(&s.shares[share], lane) = Share{top, sum};
     }
+    if (me >= shares) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     cluster.sync();
 
-    // Every block: all shares, joined to groups, and from them the beams' log-sums and the bound.
-    const int per_beam = (warps + a.join - 1) / a.join, groups = per_beam * a.beams;
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
-        const int b = g / per_beam, w0 = g % per_beam * a.join, w1 = min(w0 + a.join, warps);
-        float top = -INFINITY;
-        for (int w = w0; w < w1; ++w) top = fmaxf(top, cluster.map_shared_rank(&s.shares[b][w % kWarps], w / kWarps)->top);
-        double sum = 0;
-        for (int w = w0; w < w1; ++w) {
-            const Share h = *cluster.map_shared_rank(&s.shares[b][w % kWarps], w / kWarps);
-            sum += h.top == -INFINITY ? h.sum : h.sum * exp((double)h.top - (double)top);
-        }
-        s.group_top[g] = top;
-        s.group_sum[g] = sum;
-    }
-    __syncthreads();
+    // Every block: each beam's log-sum from its shares.
     for (int b = warp; b < a.beams; b += kWarps) {
+        const Share* of = s.shares + b * a.per_beam;
         float top = -INFINITY;
-        for (int g = lane; g < per_beam; g += 32) top = fmaxf(top, s.group_top[b * per_beam + g]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int j = lane; j < a.per_beam; j += 32) top = fmaxf(top, of[j].top);
+        top = warp_max(top);
+        const double base = base_of(top);
         double sum = 0;
-        for (int g = lane; g < per_beam; g += 32) {
-            const float t = s.group_top[b * per_beam + g];
-            sum += t == -INFINITY ? s.group_sum[b * per_beam + g] : s.group_sum[b * per_beam + g] * exp((double)t - (double)top);
-        }
+#pragma unroll 1
+        for (int j = lane; j < a.per_beam; j += 32) sum += of[j].top == -INFINITY ? of[j].sum : of[j].sum * exp2((base_of(of[j].top) - base) * (double)kLog2e);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
             const double ls = log(sum), score = a.scores[item * a.beams + b];
-            s.top[b] = top; s.log_sum[b] = ls; s.score[b] = score;
+            s.base[b] = base; s.log_sum[b] = ls; s.score[b] = score;
             s.open[b] = isfinite(top) && isfinite(ls) && isfinite(score);
         }
     }
     __syncthreads();
-    auto total = [&](int b, float x) { return s.score[b] + (((double)x - (double)s.top[b]) - s.log_sum[b]); };
+    auto total = [&](int b, float x) { return s.score[b] + (((double)x - s.base[b]) - s.log_sum[b]); };
+    // The bound: the k-th largest of the joined shares' best totals, rounded down.
+    const int groups = (shares + a.join - 1) / a.join;
     for (int g = threadIdx.x; g < groups; g += kThreads) {
-        const int b = g / per_beam;
-        s.reach[g] = s.open[b] ? __double2float_rd(total(b, s.group_top[g])) : -INFINITY;
+        float best = -INFINITY;
+        for (int i = g * a.join, end = min(i + a.join, shares); i < end; ++i) {
+            const int b = i / a.per_beam;
+            if (s.open[b] && s.shares[i].top != -INFINITY) best = fmaxf(best, __double2float_rd(total(b, s.shares[i].top)));
+        }
+        s.reach[g] = best;
     }
-    if (threadIdx.x == 0) s.bound = -INFINITY;
     __syncthreads();
     for (int g = threadIdx.x; g < groups; g += kThreads) {
         const float mine = s.reach[g];
@@ -227,89 +291,103 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(SelectArgs a) {
     const double bound = s.bound;
 
     // The shares that reach the bound, again: their totals that do.
-    for (int b = 0; b < a.beams; ++b) {
-        const float top = s.shares[b][warp].top;
-        if (s.open[b] && top != -INFINITY && total(b, top) >= bound) {
-            const T* row = rows + b * a.row_stride;
-            auto each = [&](auto&& what) {
-                for (int l = first_line(b); l < a.lines; l += warps) {
-                    float x[8];
-                    read8(row, l * kLine + lane * 8, a.vocab, a.wide, x);
+    auto reaches = [&](int share) {
+        const int b = share / a.per_beam;
+        const float top = s.shares[share].top;
+        return s.open[b] && top != -INFINITY && total(b, top) >= bound;
+    };
+    auto each = [&](int share, int turn, float least, auto&& what) {   // of a share's tokens those of the parts that reach `least`
+        const T* row = rows + share / a.per_beam * a.row_stride;
+        const unsigned parts = __ballot_sync(0xffffffffu, s.parts[turn][warp][lane] >= least);
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            if (!(parts >> (step >> shift) & 1)) continue;
+            Raw8<T> x[kLines];
+            const int line = share % a.per_beam + step * kLines * a.per_beam;
+            read(row, line, x);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) what(x[i], (unsigned)(l * kLine + lane * 8 + i));
-                }
-            };
-            int n = 0;
-            each([&](float x, unsigned) { n += x != -INFINITY && total(b, x) >= bound; });
+            for (int u = 0; u < kLines; ++u)
+                if (line + u * a.per_beam < a.lines)
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-            if (n <= a.k) {
-                each([&](float x, unsigned token) {
-                    if (x != -INFINITY && total(b, x) >= bound) {
-                        const int at = atomicAdd(&s.count, 1);
-                        s.found[at] = Found{ordered(total(b, x)), (unsigned)b * (unsigned)a.vocab + token, 0u};
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 v = x[u].two(i / 2);
+                        what(i & 1 ? v.y : v.x, (unsigned)((line + u * a.per_beam) * kLine + lane * 8 + i));
                     }
-                });
-            } else {   // many: the k best of the share, one by one
+        }
+    };
+    for (int share = me, turn = 0; share < shares; share += warps, ++turn) {
+        if (!reaches(share)) continue;
+        const int b = share / a.per_beam;
+        // a logit that may reach the bound, a little less than the one that does
+        const double from = s.base[b] + (s.log_sum[b] + (bound - s.score[b]));
+        const float least = bound == -INFINITY ? -FLT_MAX : __double2float_rd(from - fabs(from) * 1e-12 - (fabs(s.base[b]) + fabs(s.score[b]) + fabs(s.log_sum[b])) * 1e-12);
+        each(share, turn, least, [&](float x, unsigned token) {
+            if (x >= least && total(b, x) >= bound) {
+                const int at = atomicAdd(&s.count, 1);
+                if (at < kFoundCap) s.found[at] = Found{ordered(total(b, x)), (unsigned)b * (unsigned)a.vocab + token, 0u};
+            }
+        });
+    }
+    __syncthreads();
+    if (s.count > kFoundCap) {   // many totals alike: the k best of each share, one by one, and after each turn of the warps the block's k best
+        __syncthreads();
+        if (threadIdx.x == 0) s.count = 0;
+        __syncthreads();
+        for (int first = rank * kWarps, turn = 0; first < shares; first += warps, ++turn) {
+            const int share = first + warp, b = share / a.per_beam;
+            if (share < shares && reaches(share)) {
                 Found last{~0ull, 0u, 0u};
-                bool any = false;
                 for (int i = 0; i < a.k; ++i) {
                     Found best{0ull, ~0u, 0u};
-                    each([&](float x, unsigned token) {
-                        if (x == -INFINITY) return;
+                    each(share, turn, -FLT_MAX, [&](float x, unsigned token) {
                         const Found f{ordered(total(b, x)), (unsigned)b * (unsigned)a.vocab + token, 0u};
-                        if ((!any || before(last, f)) && before(f, best)) best = f;
+                        if (x != -INFINITY && (i == 0 || before(last, f)) && before(f, best)) best = f;
                     });
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) {
                         const Found f{__shfl_xor_sync(0xffffffffu, best.total, o), __shfl_xor_sync(0xffffffffu, best.at, o), 0u};
                         if (before(f, best)) best = f;
                     }
+                    if (best.total == 0) break;   // the share has no more
                     if (lane == 0) s.found[atomicAdd(&s.count, 1)] = best;
                     last = best;
-                    any = true;
                 }
             }
+            __syncthreads();
+            if (s.count > kFoundCap - kWarps * kMaxChosen) keep_best(s, a.k);
+            __syncthreads();
         }
-        // a beam adds at most kWarps * k
-        __syncthreads();
-        if (s.count > kFoundCap - kWarps * kMaxChosen) keep_best(s, a.k);
-        __syncthreads();
     }
+    __syncthreads();
     if (s.count > a.k) keep_best(s, a.k);
+    {
+        SelectShared* first = cluster.map_shared_rank(&s, 0);
+        if (threadIdx.x < s.count) first->all[rank][threadIdx.x] = s.found[threadIdx.x];
+        if (threadIdx.x == 0) first->counts[rank] = s.count;
+    }
     cluster.sync();
-
-    if (rank == 0) {
-        if (threadIdx.x == 0) {
-            int n = 0;
-            for (int r = 0; r < blocks; ++r) { s.counts[r] = n; n += *cluster.map_shared_rank(&s.count, r); }
-            s.counts[blocks] = n;
-        }
-        __syncthreads();
-        const int n = s.counts[blocks];
-        for (int i = threadIdx.x; i < blocks * kMaxChosen; i += kThreads) {
-            const int r = i / kMaxChosen, j = i % kMaxChosen;
-            if (j < s.counts[r + 1] - s.counts[r]) s.all[s.counts[r] + j] = cluster.map_shared_rank(s.found, r)[j];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const Found mine = s.all[i];
-            int place = 0;
-            for (int o = 0; o < n; ++o) place += before(s.all[o], mine);
-            if (place < a.k) {
-                const long long to = item * a.k + place;
-                a.parents[to] = (int)(mine.at / (unsigned)a.vocab);
-                a.tokens[to] = (int)(mine.at % (unsigned)a.vocab);
-                a.totals[to] = (float)from_ordered(mine.total);
-            }
-        }
-        for (int i = n + threadIdx.x; i < a.k; i += kThreads) {
-            a.parents[item * a.k + i] = -1;
-            a.tokens[item * a.k + i] = -1;
-            a.totals[item * a.k + i] = -INFINITY;
+    if (rank != 0) return;   // nobody looks into the other blocks any more
+    int n = 0;
+    for (int r = 0; r < blocks; ++r) n += s.counts[r];
+    for (int i = threadIdx.x; i < blocks * kMaxChosen; i += kThreads) {
+        const int r0 = i % blocks, j0 = i / blocks;
+        if (j0 >= s.counts[r0]) continue;
+        const Found mine = s.all[r0][j0];
+        int place = 0;
+        for (int r = 0; r < blocks; ++r)
+            for (int j = 0, end = s.counts[r]; j < end; ++j) place += before(s.all[r][j], mine);
+        if (place < a.k) {
+            const long long to = item * a.k + place;
+            a.parents[to] = (int)(mine.at / (unsigned)a.vocab);
+            a.tokens[to] = (int)(mine.at % (unsigned)a.vocab);
+            a.totals[to] = (float)from_ordered(mine.total);
         }
     }
-    cluster.sync();   // no block ends while the first reads what it found
+    for (int i = n + threadIdx.x; i < a.k; i += kThreads) {
+        a.parents[item * a.k + i] = -1;
+        a.tokens[item * a.k + i] = -1;
+        a.totals[item * a.k + i] = -INFINITY;
+    }
 }
 
 template <typename T>
@@ -319,10 +397,11 @@ psb_status select(SelectArgs a, int batch, int sms, cudaStream_t s) {
     // blocks an item: as many as fill the GPU, while each warp has a line
     int blocks = 1;
     while (blocks < kMaxCluster && (long long)batch * blocks * 2 <= 2 * sms && (long long)a.beams * a.lines >= (long long)blocks * kWarps * 2) blocks *= 2;
+    const int warps = blocks * kWarps;
+    a.per_beam = std::max(1, warps / a.beams);
     // about 8 k groups for the bound
-    const int shares = blocks * kWarps;
     a.join = 1;
-    while (a.join < shares && ((long long)shares / a.join * a.beams > kMaxGroups || (shares / (2 * a.join)) * a.beams >= 8 * a.k)) a.join *= 2;
+    while (a.per_beam * a.beams / (2 * a.join) >= 8 * a.k) a.join *= 2;
     const void* kernel = reinterpret_cast<const void*>(k_beam_select<T>);
     PSB_TRY(kernel_shared(kernel, sizeof(SelectShared)));
     if (blocks > 8) PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));

@@ -32,7 +32,8 @@ namespace cg = cooperative_groups;
 constexpr int kSlab = 128;                 // codes of a row in a slab: one swizzle row
 constexpr int kChannels = 128;             // rows of w a block
 constexpr int kMaxTokens = 256;            // rows of x a tile
-constexpr int kThreads = 192;              // four epilogue warps, one that loads, one that issues products
+constexpr int kEpilogue = 8;               // epilogue warps: two to each quarter of the tensor memory's lanes
+constexpr int kThreads = 32 * kEpilogue + 64;   // one warp loads, one issues products
 constexpr int kMaxStages = 12;
 constexpr int kRing = 200 * 1024;
 constexpr int kWaitPolls = 1 << 22;
@@ -100,6 +101,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], ready[2], drained[2], last;
     __shared__ uint32_t tmem_at;
     __shared__ int gave_up;
+    __shared__ __align__(16) float s_scales[2][kMaxTokens];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int parts = SPLIT ? (int)cg::this_cluster().num_blocks() : 1;
@@ -111,17 +113,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     constexpr int kBuffers = SPLIT ? 1 : 2;
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(&ready[i], 1); tc::mbar_init(&drained[i], 4); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&ready[i], 1); tc::mbar_init(&drained[i], kEpilogue); }
         tc::mbar_init(&last, 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 4) {
+    if (warp == kEpilogue) {
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
         }
-    } else if (warp == 5) {
+    } else if (warp == kEpilogue + 1) {
         tc::tmem_alloc(&tmem_at, tmem_columns(a.tokens, kBuffers));
     }
     tc::tc_fence_before();
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     tc::tc_fence_after();
     const uint32_t tmem = tmem_at;
 
-    if (warp == 4) {
+    if (warp == kEpilogue) {
         if (tc::elect_one()) {
             int at = 0;
             bool ok = true;
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
             }
         }
         __syncwarp();
-    } else if (warp == 5) {
+    } else if (warp == kEpilogue + 1) {
         if (tc::elect_one()) {
             const uint32_t idesc = idesc_i8(kChannels, a.tokens);
             int at = 0, count = 0;
@@ -187,29 +189,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
             if (!tc::mbar_wait(&ready[buf], (count / kBuffers) & 1, a.polls)) { gave_up = 1; break; }
             __syncwarp();
             tc::tc_fence_after();
-            const uint32_t from = tmem + buf * a.tokens + ((uint32_t)(warp * 32) << 16);
-            const int c = c0 + warp * 32 + lane;
+            const int quarter = warp & 3, half = warp >> 2;
+            const uint32_t from = tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16);
+            const int c = quarter * 32 + lane;
             if constexpr (SPLIT) {   // all products have ended: the ring is free for the partial sums, [token][channel]
                 int* partial = reinterpret_cast<int*>(ring);
-                for (int t = 0; t < a.tokens; t += 16) {
+                for (int t = half * 16; t < a.tokens; t += 32) {
                     uint32_t v[16];
                     tmem_ld16(from + t, v);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) partial[(t + i) * kChannels + warp * 32 + lane] = (int)v[i];
+                    for (int i = 0; i < 16; ++i) partial[(t + i) * kChannels + c] = (int)v[i];
                 }
             } else {
-                const float ws = c < a.n ? __ldg(a.w_scales + c) : 0.f;
-                T* out = static_cast<T*>(a.out) + c;
-                for (int t = 0; t < a.tokens && t0 + t < a.m; t += 16) {
+                float* scales = s_scales[count & 1];   // the other half still serves slower warps' last tile
+                const int i0 = warp * 32 + lane;
+                if (i0 < a.tokens) scales[i0] = t0 + i0 < a.m ? __ldg(a.x_scales + t0 + i0) : 0.f;
+                const bool here = c0 + c < a.n;
+                const float ws = here ? __ldg(a.w_scales + c0 + c) : 0.f;
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogue) : "memory");
+                T* out = static_cast<T*>(a.out) + (long long)(t0 + half * 16) * a.out_stride + c0 + c;
+                const int live = min(a.tokens, a.m - t0);
+                for (int t = half * 16; t < live; t += 32, out += 32 * a.out_stride) {
                     uint32_t v[16];
                     tmem_ld16(from + t, v);
-                    const float xs = t0 + t + (lane & 15) < a.m ? __ldg(a.x_scales + t0 + t + (lane & 15)) : 0.f;
-                    tc::tmem_ld_wait();
+                    float by[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float by = __shfl_sync(0xffffffffu, xs, i);
-                        if (c < a.n && t0 + t + i < a.m) out[(long long)(t0 + t + i) * a.out_stride] = rounded<T>((float)(int)v[i] * by * ws);
+                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(by + i) = *reinterpret_cast<const float4*>(scales + t + i);
+                    tc::tmem_ld_wait();
+                    if (here) {
+                        T* to = out;
+                        if (t + 16 <= live) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i, to += a.out_stride) *to = rounded<T>((float)(int)v[i] * by[i] * ws);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i, to += a.out_stride)
+                                if (t + i < live) *to = rounded<T>((float)(int)v[i] * by[i] * ws);
+                        }
                     }
                 }
                 tc::tc_fence_before();
@@ -221,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    if (warp == 5) tc::tmem_dealloc(tmem, tmem_columns(a.tokens, kBuffers));
+    if (warp == kEpilogue + 1) tc::tmem_dealloc(tmem, tmem_columns(a.tokens, kBuffers));
 
     if constexpr (SPLIT) {
         cg::cluster_group cluster = cg::this_cluster();
@@ -231,8 +248,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
         const int c0 = first % a.channel_tiles * kChannels, t0 = first / a.channel_tiles * a.tokens;
         const int* partial = reinterpret_cast<const int*>(ring);
         // four channels a thread: 32 threads a token
+        constexpr int kWarps = kThreads / 32;
         const int c4 = (threadIdx.x & 31) * 4;
-        for (int t = part * 6 + warp; t < a.tokens && t0 + t < a.m; t += 6 * parts) {
+        for (int t = part * kWarps + warp; t < a.tokens && t0 + t < a.m; t += kWarps * parts) {
             int s[4] = {0, 0, 0, 0};
             if (!lost) {
                 for (int p = 0; p < parts; ++p) {

@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -31,8 +33,39 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
-template <int VEC> struct alignas(VEC) Codes { signed char v[VEC]; };
+// VEC neighbouring elements: one, or 16 bytes.
+template <typename T, int VEC> struct Pack {
+    static_assert(VEC * sizeof(T) == 16, "16 bytes or one element");
+    unsigned word[4];
+    __device__ __forceinline__ void read(const T* at) { set(*reinterpret_cast<const uint4*>(at)); }
+    // a second time, rather than held in registers
+    __device__ __forceinline__ void read_again(const T* at) {
+        asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(word[0]), "=r"(word[1]), "=r"(word[2]), "=r"(word[3]) : "l"(at));
+    }
+    __device__ __forceinline__ void set(uint4 v) { word[0] = v.x; word[1] = v.y; word[2] = v.z; word[3] = v.w; }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(word[e]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e & 1 ? word[e >> 1] & 0xffff0000u : word[e >> 1] << 16);
+        else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&word[e >> 1])); return e & 1 ? f.y : f.x; }
+    }
+    static __device__ __forceinline__ void write(T* at, const float (&v)[VEC]) {
+        unsigned o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) o[i] = __float_as_uint(v[i]);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) { const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); o[i] = *reinterpret_cast<const unsigned*>(&p); }
+            else { const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]); o[i] = *reinterpret_cast<const unsigned*>(&p); }
+        }
+        *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+};
+template <typename T> struct Pack<T, 1> {
+    float v;
+    __device__ __forceinline__ void read(const T* at) { v = to_float(*at); }
+    __device__ __forceinline__ void read_again(const T* at) { v = to_float(*at); }
+    __device__ __forceinline__ float get(int) const { return v; }
+    static __device__ __forceinline__ void write(T* at, const float (&v)[1]) { *at = from_float<T>(v[0]); }
+};
 
 struct RowArgs {
     const void* x;
@@ -46,133 +79,201 @@ struct RowArgs {
     float eps;
 };
 
-// Reductions over the TPR threads of a row.  Every thread of the block takes part; `slots` holds a value a warp.
-template <int TPR, typename V, typename Op>
-__device__ __forceinline__ V row_reduce(V v, V* slots, Op op) {
-#pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) >> 1; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if constexpr (TPR > 32) {
-        if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = slots[threadIdx.x & 31 & (TPR / 32 - 1)];
-#pragma unroll
-        for (int o = TPR / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-        __syncthreads();
-    }
-    return v;
-}
 struct MaxOp { template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct SumOp { template <typename V> __device__ V operator()(V a, V b) const { return a + b; } };
 
+template <int WIDTH, typename V, typename Op>
+__device__ __forceinline__ V lanes_reduce(V v, Op op) {
+#pragma unroll
+    for (int o = WIDTH >> 1; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+// Over the THREADS threads of a block.  `slots` holds a value a warp and is used once.
+template <int THREADS, typename V, typename Op>
+__device__ __forceinline__ V block_reduce(V v, V* slots, Op op) {
+    v = lanes_reduce<32>(v, op);
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return lanes_reduce<THREADS / 32>(slots[threadIdx.x & (THREADS / 32 - 1)], op);
+}
+
 // A magnitude's bits: their order as integers is that of the magnitudes, and a NaN's are above all.
-__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ unsigned long long magnitude(double v) { return (unsigned long long)__double_as_longlong(v) & 0x7fffffffffffffffull; }
+// The larger magnitude; NaN where either is.
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+struct LargerOp { __device__ float operator()(float a, float b) const { return larger(a, b); } };
 
 __device__ __forceinline__ signed char code64(double u, double top) { return (signed char)(int)rint(127.0 * u / top); }
 
-// What a row's reductions gave.
-struct RowTop { double top; float inverse; bool wild, dead; };
+constexpr float kRint = 12582912.f;   // 1.5 * 2^23: a sum with it is rounded to whole numbers, which its lowest bits hold
 
-// One row for each group of TPR threads, in registers: at most NV packs of VEC elements a thread.
+// Four codes' lowest bytes in one word.
+__device__ __forceinline__ unsigned four(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// One row for each group of TPR threads, in registers: at most NV packs of VEC elements a thread.  What few elements need - 64 bits next to
+// ties, at the top, in rows out of fp32's range - is read again from memory, before the sum is written, by the 32 lanes of a warp for the one
+// that found it.  Code for it beside every element took five times the kernel's time, and a thread of its own for it half of the rest, the
+// block waiting (16,384 rows of 8,192 in bf16: 789 and 499 us).
 template <typename T, int VEC, int NV, int TPR, bool NORM>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_i8_rows(RowArgs a) {
     constexpr int kThreads = TPR < 256 ? 256 : TPR;
-    constexpr int kSlots = kThreads / 32;
     using P = Pack<T, VEC>;
-    // one set of slots for each group of TPR threads
-    __shared__ float s_sum[kSlots];
-    __shared__ unsigned s_top[kSlots];
-    __shared__ unsigned long long s_top64[kSlots];
-    __shared__ double s_sum64[kSlots];
     static_assert(TPR <= 32 || TPR == kThreads, "a row's threads are part of a warp or the whole block");
-    const int lane = threadIdx.x % TPR;
+    static_assert(NV * VEC <= 32, "a warp takes a lane's elements at once");
+    __shared__ float s_sum[kThreads / 32], s_top[kThreads / 32];
+    __shared__ unsigned long long s_top64[kThreads / 32];
+    __shared__ double s_sum64[kThreads / 32];
+    const int lane = threadIdx.x % TPR, lane32 = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * (kThreads / TPR) + threadIdx.x / TPR;
     const bool live = row < a.n;
-    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
-    const T* r = NORM && a.residual ? static_cast<const T*>(a.residual) + (live ? row : 0) * a.residual_stride : nullptr;
     const T* w = NORM ? static_cast<const T*>(a.weight) : nullptr;
-    P px[NV], pr[NV], pw[NV];
+    const int dim = live ? a.dim : 0;
+    float h[NV][VEC];   // the row, or its sum with the residual
+    float sum = 0.f, mine = 0.f;
+    {
+        const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
+        const T* r = NORM && a.residual ? static_cast<const T*>(a.residual) + (live ? row : 0) * a.residual_stride : nullptr;
+        P px[NV], pr[NORM ? NV : 1], pw[NORM ? NV : 1];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int at = (j * TPR + lane) * VEC;
-        const bool in = live && at < a.dim;
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * TPR + lane) * VEC;
+            if (at < dim) {
+                px[j].read(x + at);
+                if (NORM && r) pr[j].read(r + at);
+                if (NORM && w) pw[j].read(w + at);
+            }
+        }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { px[j].v[e] = from_float<T>(0.f); pr[j].v[e] = from_float<T>(0.f); pw[j].v[e] = from_float<T>(1.f); }
-        if (in) {
-            px[j] = *reinterpret_cast<const P*>(x + at);
-            if (NORM) {
-                if (r) pr[j] = *reinterpret_cast<const P*>(r + at);
-                if (w) pw[j] = *reinterpret_cast<const P*>(w + at);
+        for (int j = 0; j < NV; ++j) {
+            const bool in = (j * TPR + lane) * VEC < dim;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                h[j][e] = in ? px[j].get(e) : 0.f;
+                if (NORM) {
+                    if (r && in) h[j][e] += pr[j].get(e);
+                    sum = fmaf(h[j][e], h[j][e], sum);
+                }
+                mine = larger(mine, NORM && w && in ? h[j][e] * pw[j].get(e) : h[j][e]);
             }
         }
     }
-    auto value = [&](int j, int e) { return NORM ? (to_float(px[j].v[e]) + to_float(pr[j].v[e])) * to_float(pw[j].v[e]) : to_float(px[j].v[e]); };
-    auto value64 = [&](int j, int e) {
-        return NORM ? ((double)to_float(px[j].v[e]) + (double)to_float(pr[j].v[e])) * (double)to_float(pw[j].v[e]) : (double)to_float(px[j].v[e]);
-    };
-    float sum = 0.f;
-    unsigned top = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            if (NORM) { const float h = to_float(px[j].v[e]) + to_float(pr[j].v[e]); sum = fmaf(h, h, sum); }
-            top = max(top, magnitude(value(j, e)));
-        }
-    top = row_reduce<TPR>(top, s_top, MaxOp());
-    if (NORM) sum = row_reduce<TPR>(sum, s_sum, SumOp());
-    const float top32 = __uint_as_float(top);
+    float top32 = mine;
+    if constexpr (TPR <= 32) {
+        top32 = lanes_reduce<TPR>(top32, LargerOp());
+        if (NORM) sum = lanes_reduce<TPR>(sum, SumOp());
+    } else {
+        top32 = lanes_reduce<32>(top32, LargerOp());
+        if (NORM) sum = lanes_reduce<32>(sum, SumOp());
+        if (lane32 == 0) { s_top[threadIdx.x >> 5] = top32; s_sum[threadIdx.x >> 5] = sum; }
+        __syncthreads();
+        top32 = lanes_reduce<kThreads / 32>(s_top[threadIdx.x & (kThreads / 32 - 1)], LargerOp());
+        if (NORM) sum = lanes_reduce<kThreads / 32>(s_sum[threadIdx.x & (kThreads / 32 - 1)], SumOp());
+    }
     // (a NaN fails every comparison; a row without a norm has no sum to look at)
-    const bool wild = !(top32 >= kSafeLow && top32 <= kSafeHigh) || (NORM && !(sum >= kSafeLow && sum <= kSafeHigh));
+    bool wild = !(top32 >= kSafeLow && top32 <= kSafeHigh) || (NORM && !(sum >= kSafeLow && sum <= kSafeHigh));
+    if (TPR > 32 ? top32 == 0.f : __any_sync(0xffffffffu, top32 == 0.f)) {   // perhaps a row of zeros
+        bool some = false;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) some = some || h[j][e] != 0.f;
+        some = TPR > 32 ? __syncthreads_or(some) : lanes_reduce<(TPR < 32 ? TPR : 32)>((int)some, MaxOp());
+        if (top32 == 0.f && !some) wild = false;
+    }
+
+    // For each lane of the warp that needs it: f(lane, its row, element of the row, its value in 32 bits, its sum and value in 64), an element
+    // of that lane's for each of the 32 (an element < 0: none).
+    auto together = [&](bool need, auto&& f) {
+        __syncwarp();   // what f writes lies over what its lane wrote, what it reads under what that writes next
+        for (unsigned todo = __ballot_sync(0xffffffffu, need && live); todo; todo &= todo - 1) {
+            const int whose = __ffs(todo) - 1;
+            const long long of = __shfl_sync(0xffffffffu, row, whose);
+            const int l = TPR <= 32 ? whose % TPR : (int)(threadIdx.x & ~31u) + whose;
+            int i = (lane32 / VEC * TPR + l) * VEC + lane32 % VEC;
+            if (lane32 >= NV * VEC || i >= a.dim) i = -1;
+            float v = 0.f;
+            double s64 = 0, v64 = 0;
+            if (i >= 0) {
+                const float x = to_float(static_cast<const T*>(a.x)[of * a.x_stride + i]);
+                const float r = NORM && a.residual ? to_float(static_cast<const T*>(a.residual)[of * a.residual_stride + i]) : 0.f;
+                const float by = NORM && w ? to_float(w[i]) : 1.f;
+                v = NORM ? (x + r) * by : x;
+                s64 = (double)x + (double)r;
+                v64 = s64 * (double)by;
+            }
+            f(whose, of, i, v, s64, v64);
+        }
+        __syncwarp();
+    };
     double top64 = top32, mean = NORM ? (double)sum / a.dim : 0;
-    // The whole block takes the 64-bit reductions where a row of it needs them.
+    // the whole warp or block takes the 64-bit reductions where a row of it needs them
     const bool any_wild = TPR > 32 ? wild : __any_sync(0xffffffffu, wild);
     if (NORM || any_wild) {
         unsigned long long t = 0;
-        const float near = wild ? -1.f : top32 * kNearTop;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (wild || fabsf(value(j, e)) >= near) t = max(t, magnitude(value64(j, e)));
-        top64 = __longlong_as_double((long long)row_reduce<TPR>(t, s_top64, MaxOp()));
+        const float near = top32 * kNearTop;
+        together(wild || mine >= near, [&](int whose, long long, int, float v, double, double v64) {
+            const bool all = __shfl_sync(0xffffffffu, (int)wild, whose);
+            const float least = __shfl_sync(0xffffffffu, near, whose);
+            const unsigned long long m = lanes_reduce<32>(all || fabsf(v) >= least ? magnitude(v64) : 0ull, MaxOp());
+            if (lane32 == whose) t = m;
+        });
+        t = TPR <= 32 ? lanes_reduce<(TPR < 32 ? TPR : 32)>(t, MaxOp()) : block_reduce<kThreads>(t, s_top64, MaxOp());
+        top64 = __longlong_as_double((long long)t);
     }
     if (NORM && any_wild) {
         double s = 0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) { const double h = (double)to_float(px[j].v[e]) + (double)to_float(pr[j].v[e]); s = fma(h, h, s); }
-        s = row_reduce<TPR>(s, s_sum64, SumOp());
+        together(wild, [&](int whose, long long, int, float, double s64, double) {
+            const double m = lanes_reduce<32>(s64 * s64, SumOp());
+            if (lane32 == whose) s = m;
+        });
+        s = TPR <= 32 ? lanes_reduce<(TPR < 32 ? TPR : 32)>(s, SumOp()) : block_reduce<kThreads>(s, s_sum64, SumOp());
         if (wild) mean = s / a.dim;
     }
-    if (!live) return;
     const bool dead = !(top64 <= 1.7e308) || (NORM && !(mean <= 1.7e308));   // an infinity or a NaN: no codes, and a scale that says so
-    if (lane == 0) {
-        const double by = NORM ? 127.0 * sqrt(mean + (double)a.eps) : 127.0;
-        a.scales[row] = dead ? __int_as_float(0x7fffffff) : top64 > 0 ? (float)(top64 / by) : 0.f;
-    }
-    const float inverse = 127.f / (float)top64;
-    signed char* out = a.codes + row * a.code_stride;
+    const float inverse = top64 > 0 ? 127.f / (float)top64 : 0.f;
+    signed char* out = a.codes + (live ? row : 0) * a.code_stride;
+    float off = 0.f;   // the furthest from a whole number
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int at = (j * TPR + lane) * VEC;
-        if (at >= a.dim) continue;
-        Codes<VEC> c;
+        if (at >= dim) continue;
+        P pw;
+        if (NORM && w) pw.read_again(w + at);
+        unsigned c[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const float t = value(j, e) * inverse, q = rintf(t);
-            int code = (int)q;
-            if (wild || fabsf(t - q) > kNearTie) code = dead || top64 == 0 ? 0 : code64(value64(j, e), top64);
-            c.v[e] = (signed char)code;
+            const float t = (NORM && w ? h[j][e] * pw.get(e) : h[j][e]) * inverse, m = t + kRint;
+            c[e] = __float_as_uint(m);
+            off = fmaxf(off, fabsf(t - (m - kRint)));
         }
-        *reinterpret_cast<Codes<VEC>*>(out + at) = c;
-        if (NORM && a.sum) {
-            P s;
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(out + at) = make_uint2(four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7]));
+        else if constexpr (VEC == 4) *reinterpret_cast<unsigned*>(out + at) = four(c[0], c[1], c[2], c[3]);
+        else out[at] = (signed char)c[0];
+    }
+    together(wild || off > kNearTie, [&](int whose, long long of, int i, float v, double, double v64) {
+        const bool all = __shfl_sync(0xffffffffu, (int)wild, whose), none = __shfl_sync(0xffffffffu, (int)dead, whose);
+        const double top = __shfl_sync(0xffffffffu, top64, whose);
+        const float t = v * __shfl_sync(0xffffffffu, inverse, whose);
+        if (i >= 0 && (all || fabsf(t - ((t + kRint) - kRint)) > kNearTie)) a.codes[of * a.code_stride + i] = none || top == 0 ? (signed char)0 : code64(v64, top);
+    });
+    if (NORM && a.sum) {
+        T* to = static_cast<T*>(a.sum) + (live ? row : 0) * a.sum_stride;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s.v[e] = from_float<T>(to_float(px[j].v[e]) + to_float(pr[j].v[e]));
-            *reinterpret_cast<P*>(static_cast<T*>(a.sum) + row * a.sum_stride + at) = s;
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * TPR + lane) * VEC;
+            if (at >= dim) continue;
+            P::write(to + at, h[j]);
         }
+    }
+    if (live && lane == 0) {
+        const double by = NORM ? 127.0 * sqrt(mean + (double)a.eps) : 127.0;
+        a.scales[row] = dead ? __int_as_float(0x7fffffff) : top64 > 0 ? (float)(top64 / by) : 0.f;
     }
 }
 
@@ -194,8 +295,8 @@ __global__ void __launch_bounds__(1024) k_i8_rows_long(RowArgs a) {
         if (NORM) sum = fma(h, h, sum);
         t = max(t, magnitude(w ? h * (double)to_float(w[i]) : h));
     }
-    const double top = __longlong_as_double((long long)row_reduce<1024>(t, s_top64, MaxOp()));
-    const double mean = NORM ? row_reduce<1024>(sum, s_sum64, SumOp()) / a.dim : 0;
+    const double top = __longlong_as_double((long long)block_reduce<1024>(t, s_top64, MaxOp()));
+    const double mean = NORM ? block_reduce<1024>(sum, s_sum64, SumOp()) / a.dim : 0;
     const bool dead = !(top <= 1.7e308) || !(mean <= 1.7e308);
     if (threadIdx.x == 0) {
         const double by = NORM ? 127.0 * sqrt(mean + (double)a.eps) : 127.0;
@@ -219,15 +320,15 @@ psb_status start(const RowArgs& a, cudaStream_t s) {
     return PSB_OK;
 }
 
-// Threads a row: the fewest whose registers hold it; more where rows are too few to fill the GPU.
-template <typename T, int VEC, int NV, bool NORM>
+// Threads a row: the fewest whose registers hold it, 16 elements each; more where rows are too few to fill the GPU.
+template <typename T, int VEC, bool NORM>
 psb_status by_length(const RowArgs& a, int sms, cudaStream_t s) {
-    constexpr int each = VEC * NV;
+    constexpr int NV = 16 / VEC;
     int tpr = 8;
-    if (a.dim > 8 * each) tpr = 32;
-    if (a.dim > 32 * each) tpr = 256;
-    if (a.dim > 256 * each) tpr = 512;
-    if (a.dim > 512 * each) tpr = 1024;
+    if (a.dim > 8 * 16) tpr = 32;
+    if (a.dim > 32 * 16) tpr = 256;
+    if (a.dim > 256 * 16) tpr = 512;
+    if (a.dim > 512 * 16) tpr = 1024;
     while (tpr < 1024 && a.dim > tpr * VEC && a.n * tpr < (long long)sms * 1024) tpr = tpr == 8 ? 32 : tpr == 32 ? 256 : 2 * tpr;
     switch (tpr) {
         case 8: return start<T, VEC, NV, 8, NORM>(a, s);
@@ -244,8 +345,7 @@ psb_status by_layout(const RowArgs& a, int sms, cudaStream_t s) {
     auto at = [](const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; };
     const bool wide = a.dim % VEC == 0 && at(a.x, 16) && a.x_stride % VEC == 0 && at(a.codes, VEC) && a.code_stride % VEC == 0 &&
                       (!a.residual || (at(a.residual, 16) && a.residual_stride % VEC == 0)) && (!a.sum || (at(a.sum, 16) && a.sum_stride % VEC == 0)) && at(a.weight, 16);
-    if (wide && a.dim <= 1024 * VEC * 4) return by_length<T, VEC, 4, NORM>(a, sms, s);
-    if (a.dim <= 1024 * 16) return by_length<T, 1, 16, NORM>(a, sms, s);
+    if (a.dim <= 1024 * 16) return wide ? by_length<T, VEC, NORM>(a, sms, s) : by_length<T, 1, NORM>(a, sms, s);
     k_i8_rows_long<T, NORM><<<(unsigned)a.n, 1024, 0, s>>>(a);
     PSB_LAUNCH_CHECK();
     count_launch();
