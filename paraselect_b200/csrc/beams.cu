@@ -3,9 +3,9 @@
 //
 // Selection.  total(beam, token) = score + log p, log p = (x - max) - log sum exp(x - max); the k largest totals of an item, ties to the
 // lowest (beam, token).  One cluster of blocks takes an item, and the logits are read once: a warp reduces its share of a beam's row to a
-// maximum and a sum.  From those every block has each beam's log-sum, and a bound: of all shares' maxima, as totals, the k-th largest - at
-// least k totals reach it.  Only shares whose maximum reaches the bound, hardly more than k of them, are looked through again for the totals
-// that do; the few found are ranked by the cluster's first block.  Sums are held in fp32 within a lane (some hundred terms) and in 64 bits
+// maximum and a sum, and to the maxima of groups of its lanes.  From those every block has each beam's log-sum, and a bound that k of the
+// groups' maxima, as totals, reach, so that at least k totals do.  Only the parts of a share whose maximum reaches the bound are looked through
+// again; the few totals found are ranked by the cluster's first block.  Sums are held in fp32 within a lane (some hundred terms) and in 64 bits
 // beyond, totals are compared in 64 bits.  The warps of a cluster are dealt out to the beams, so that a warp of a small call waits for one
 // round of loads and reduces once.
 //
@@ -33,6 +33,7 @@ constexpr int kMaxBeams = 64;
 constexpr int kMaxChosen = 64;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxShares = kMaxCluster * kWarps;
+constexpr int kMaxGroups = 2 * kThreads;   // groups of lanes, for the bound
 constexpr int kFoundCap = 2048;
 
 struct SelectArgs {
@@ -44,9 +45,14 @@ struct SelectArgs {
     long long row_stride;
     int beams, vocab, k, lines;
     int per_beam;                       // warps that share a beam's row; share s is part s % per_beam of beam s / per_beam, and its warp's (s / warps)-th
-    int join;                           // shares joined for the bound
+    unsigned by_beam;                   // 2^32 / per_beam, rounded up
+    int groups;                         // of a share's lanes: a power of two
     bool wide;                          // rows begin at multiples of 16 bytes
 };
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // 2^v to 2 units in the last place; results below 2^-126 are zero, which a sum of one or more does not notice.
 __device__ __forceinline__ float exp2_of(float v) {
@@ -87,7 +93,23 @@ __device__ __forceinline__ float warp_max(float v) {
 // Eight neighbouring tokens' logits as they lie in memory; -inf behind the vocabulary's end.
 template <typename T> struct Raw8 {
     static constexpr int kWords = 2 * sizeof(T);
+    static constexpr unsigned kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;   // -inf
     unsigned word[kWords];
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) word[i] = kNone;
+    }
+    // The largest of two words' logits, in pairs where a word holds two.
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+        if constexpr (sizeof(T) == 4) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+        else if constexpr (std::is_same<T, __half>::value) { const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b)); return *reinterpret_cast<const unsigned*>(&m); }
+        else { const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b)); return *reinterpret_cast<const unsigned*>(&m); }
+    }
+    static __device__ __forceinline__ float largest(unsigned m) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+        else if constexpr (std::is_same<T, __half>::value) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m)); return fmaxf(f.x, f.y); }
+        else return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+    }
     __device__ __forceinline__ void read(const T* row, int at, int vocab, bool wide) {
         if (wide && at + 8 <= vocab) {
 #pragma unroll
@@ -125,23 +147,41 @@ __device__ __forceinline__ double from_ordered(unsigned long long o) { return __
 struct Found { unsigned long long total; unsigned at; unsigned pad; };   // at = beam * vocab + token
 __device__ __forceinline__ bool before(const Found& a, const Found& b) { return a.total > b.total || (a.total == b.total && a.at < b.at); }
 
-// The largest logit, and the sum of exp2((x - base) kLog2e) over the share's tokens.  base = (top kLog2e) / kLog2e with the product rounded to fp32,
+// The largest logit, and the sum of exp2((x - base) kLog2e) over the share's tokens.  base = (top kLog2e) (1 / kLog2e) with the product rounded to fp32,
 // so that an exponent takes one fused operation and what the rounding changed is known; where that product leaves fp32, the logit itself.
 struct Share { float top; double sum; };
 __device__ __forceinline__ bool huge(float top) { return fabsf(top) > 1e38f; }
-__device__ __forceinline__ double base_of(float top) { return huge(top) ? (double)top : (double)(top * kLog2e) / (double)kLog2e; }
+__device__ __forceinline__ double base_of(float top) { return huge(top) ? (double)top : (double)(top * kLog2e) * (1.0 / (double)kLog2e); }
+
+// 2^v for v <= 0 with a relative error below 1e-9: the Taylor series of e^(f ln 2), |f| <= 1/2, to the eighth power.  (CUDA's own, exact to the last of
+// 53 bits, took a quarter of a small call's time.)
+__device__ __forceinline__ double exp2_64(double v) {
+    if (!(v > -1000.0)) return v == v ? 0.0 : v;
+    const double n = rint(v), f = (v - n) * 0.69314718055994531;
+    double p = 1.0 / 40320;
+    p = fma(p, f, 1.0 / 5040); p = fma(p, f, 1.0 / 720); p = fma(p, f, 1.0 / 120); p = fma(p, f, 1.0 / 24);
+    p = fma(p, f, 1.0 / 6); p = fma(p, f, 0.5); p = fma(p, f, 1.0); p = fma(p, f, 1.0);
+    return p * __longlong_as_double((long long)((int)n + 1023) << 52);
+}
+// log v for 1/2 <= v <= 2^25, in fp32 and one step of Newton's method on e^y = v, whose error is the square of fp32's.
+__device__ __forceinline__ double log_64(double v) {
+    const double y = (double)logf((float)v), e = v * exp2_64(-y * 1.4426950408889634) - 1.0;
+    return y + (e - 0.5 * e * e);
+}
 
 struct SelectShared {
     Share shares[kMaxShares];                        // of the whole item, written by their warps in every block
-    float parts[kMaxBeams / kWarps][kWarps][32];     // the largest logits of 32 parts of this block's shares
+    // of this block's shares: the largest logits of 32 parts, and of each lane's steps the three largest, with the numbers of two
+    float parts[kMaxBeams / kWarps][kWarps][32];
+    float4 steps[kMaxBeams / kWarps][kWarps][32];
     Found found[kFoundCap];
     int count;
-    float reach[kMaxShares];
+    float tops[kMaxGroups];                          // of the groups of lanes of all shares, as `shares`
+    float most[kWarps];
     double base[kMaxBeams], log_sum[kMaxBeams], score[kMaxBeams];
     bool open[kMaxBeams];                            // the beam offers continuations
-    float bound;
     Found all[kMaxCluster][kMaxChosen];              // in the cluster's first block: what every block found
-    int counts[kMaxCluster];
+    int counts[kMaxCluster], first[kMaxCluster + 1];
 };
 
 // The found ones beyond the k best go; the k best stay in no order.  For all threads of the block.
@@ -178,7 +218,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int warps = blocks * kWarps, me = rank * kWarps + warp, shares = a.per_beam * a.beams;
     const T* rows = static_cast<const T*>(a.logits) + item * a.beams * a.row_stride;
-    if (threadIdx.x == 0) { s.count = 0; s.bound = -INFINITY; }
+    auto beam_of = [&](int share) { return a.per_beam == 1 ? share : (int)__umulhi((unsigned)share, a.by_beam); };   // exact: shares are below 2^16
+    auto part_of = [&](int share) { return share - beam_of(share) * a.per_beam; };
+    if (threadIdx.x == 0) s.count = 0;
+    if (threadIdx.x < a.beams) s.score[threadIdx.x] = a.scores[item * a.beams + threadIdx.x];
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // waited for before the first write to another block
 
     // A share's lines are per_beam apart, kLines of them at a time, read ahead by as many.
@@ -188,25 +231,34 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
     while ((steps - 1) >> shift >= 32) ++shift;
     auto read = [&](const T* row, int line, Raw8<T> (&x)[kLines]) {
 #pragma unroll
-        for (int u = 0; u < kLines; ++u)
+        for (int u = 0; u < kLines; ++u) {
             if (line + u * a.per_beam < a.lines) x[u].read(row, (line + u * a.per_beam) * kLine + lane * 8, a.vocab, a.wide);
+            else x[u].none();
+        }
     };
     for (int share = me, turn = 0; share < shares; share += warps, ++turn) {
-        const T* row = rows + share / a.per_beam * a.row_stride;
+        const T* row = rows + beam_of(share) * a.row_stride;
         float top = -INFINITY, at = 0.f, part = -INFINITY;
+        float best = -INFINITY, second = -INFINITY, third = -INFINITY;   // of this lane's steps
+        unsigned which = 0;                                             // best's number in the low half, second's in the high
         unsigned long long sums = 0;   // two sums of zero
         Raw8<T> x[kLines], next[kLines];
-        int line = share % a.per_beam;
+        int line = part_of(share);
         read(row, line, x);
+#pragma unroll 2
         for (int step = 0; step < steps; ++step, line += kLines * a.per_beam) {
             if (step + 1 < steps) read(row, line + kLines * a.per_beam, next);
-            float t = -INFINITY;
+            unsigned m = Raw8<T>::kNone;
 #pragma unroll
             for (int u = 0; u < kLines; ++u)
-                if (line + u * a.per_beam < a.lines)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { const float2 v = x[u].two(i); t = fmaxf(t, fmaxf(v.x, v.y)); }
+                for (int i = 0; i < Raw8<T>::kWords; ++i) m = Raw8<T>::larger(m, x[u].word[i]);
+            const float t = Raw8<T>::largest(m);
             const float most = warp_max(t);
+            which = t > best ? which << 16 | (unsigned)step : t > second ? (which & 0xffffu) | (unsigned)step << 16 : which;
+            third = t > second ? second : fmaxf(third, t);
+            second = t > best ? best : fmaxf(second, t);
+            best = fmaxf(best, t);
             if (lane == step >> shift) part = fmaxf(part, most);
             if (most > top) {   // the same for all lanes: the sums come down to the new base
                 const float to = most * kLog2e;
@@ -228,12 +280,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
                 const unsigned long long scale = pair(kLog2e, kLog2e), less = pair(-at, -at);
 #pragma unroll
                 for (int u = 0; u < kLines; ++u)
-                    if (line + u * a.per_beam < a.lines)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 v = x[u].two(i), e = halves(fma2(pair(v.x, v.y), scale, less));
-                            sums = add2(sums, pair(exp2_of(e.x), exp2_of(e.y)));
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 v = x[u].two(i), e = halves(fma2(pair(v.x, v.y), scale, less));
+                        sums = add2(sums, pair(exp2_of(e.x), exp2_of(e.y)));
+                    }
             }
 #pragma unroll
             for (int u = 0; u < kLines; ++u) x[u] = next[u];
@@ -244,8 +295,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         s.parts[turn][warp][lane] = part;
+        s.steps[turn][warp][lane] = make_float4(best, second, third, __uint_as_float(which));
         if (turn == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        for (int o = 16; o >= a.groups; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
         if (lane < blocks) *cluster.map_shared_rank(&s.shares[share], lane) = Share{top, sum};
+        if (lane < a.groups)
+            for (int r = 0; r < blocks; ++r) *cluster.map_shared_rank(&s.tops[share * a.groups + lane], r) = best;
     }
     if (me >= shares) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     cluster.sync();
@@ -259,74 +314,100 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
         const double base = base_of(top);
         double sum = 0;
 #pragma unroll 1
-        for (int j = lane; j < a.per_beam; j += 32) sum += of[j].top == -INFINITY ? of[j].sum : of[j].sum * exp2((base_of(of[j].top) - base) * (double)kLog2e);
+        for (int j = lane; j < a.per_beam; j += 32) sum += of[j].top == -INFINITY ? of[j].sum : of[j].sum * exp2_64((base_of(of[j].top) - base) * (double)kLog2e);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
-            const double ls = log(sum), score = a.scores[item * a.beams + b];
-            s.base[b] = base; s.log_sum[b] = ls; s.score[b] = score;
-            s.open[b] = isfinite(top) && isfinite(ls) && isfinite(score);
+            s.base[b] = base; s.log_sum[b] = log_64(sum);
+            s.open[b] = isfinite(top) && isfinite(sum) && isfinite(s.score[b]);
         }
     }
     __syncthreads();
     auto total = [&](int b, float x) { return s.score[b] + (((double)x - s.base[b]) - s.log_sum[b]); };
-    // The bound: the k-th largest of the joined shares' best totals, rounded down.
-    const int groups = (shares + a.join - 1) / a.join;
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
-        float best = -INFINITY;
-        for (int i = g * a.join, end = min(i + a.join, shares); i < end; ++i) {
-            const int b = i / a.per_beam;
-            if (s.open[b] && s.shares[i].top != -INFINITY) best = fmaxf(best, __double2float_rd(total(b, s.shares[i].top)));
+    // The bound.  Totals rounded down, so that where k of these reach it, so do k totals.
+    const int groups = shares * a.groups;
+    float mine[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int g = threadIdx.x + i * kThreads, b = beam_of(min(g, groups - 1) / a.groups);
+        mine[i] = g < groups && s.open[b] && s.tops[g] != -INFINITY ? __double2float_rd(total(b, s.tops[g])) : -INFINITY;
+    }
+    float most = warp_max(fmaxf(mine[0], mine[1]));
+    if (lane == 0) s.most[warp] = most;
+    auto reach = [&](float least) { return __syncthreads_count(mine[0] >= least) + (groups > kThreads ? __syncthreads_count(mine[1] >= least) : 0); };
+    float low = -INFINITY;
+    if (reach(-FLT_MAX) >= a.k) {
+        most = warp_max(s.most[lane & (kWarps - 1)]);
+        // steps down from the largest until k reach it, then halves of the last step while many more do
+        float high = most, down = 2.f;
+        low = most - down;
+        int n = reach(low);
+        while (n < a.k && low > -FLT_MAX) { high = low; down *= 2.f; low = fmaxf(most - down, -FLT_MAX); n = reach(low); }
+        for (int i = 0; i < 8 && n > a.k + 1 + a.k / 4; ++i) {
+            const float mid = 0.5f * low + 0.5f * high;
+            if (!(mid > low && mid < high)) break;
+            const int m = reach(mid);
+            if (m >= a.k) { low = mid; n = m; } else high = mid;
         }
-        s.reach[g] = best;
     }
-    __syncthreads();
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
-        const float mine = s.reach[g];
-        int above = 0;
-        for (int o = 0; o < groups; ++o) above += s.reach[o] > mine || (s.reach[o] == mine && o < g);
-        if (above == a.k - 1) s.bound = mine;
-    }
-    __syncthreads();
-    const double bound = s.bound;
+    const double bound = low;
 
     // The shares that reach the bound, again: their totals that do.
     auto reaches = [&](int share) {
-        const int b = share / a.per_beam;
+        const int b = beam_of(share);
         const float top = s.shares[share].top;
         return s.open[b] && top != -INFINITY && total(b, top) >= bound;
     };
+    // what(logit, token) for those of this lane's tokens in a step that reach `least`.  Few do: a mask of them first, then one after the other, so that
+    // the code for one is not laid out for every token (instructions that are fetched once cost a small call more than what they do).
+    auto few = [&](const T* row, int line, float least, auto&& what) {
+        Raw8<T> x[kLines];
+        read(row, line, x);
+        unsigned mask = 0;
+#pragma unroll
+        for (int u = 0; u < kLines; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = x[u].two(i);
+                mask |= (unsigned)(v.x >= least) << (8 * u + 2 * i) | (unsigned)(v.y >= least) << (8 * u + 2 * i + 1);
+            }
+#pragma unroll 1
+        for (; mask; mask &= mask - 1) {
+            const int bit = __ffs(mask) - 1, token = (line + (bit >> 3) * a.per_beam) * kLine + lane * 8 + (bit & 7);
+            what(to_float(row[token]), (unsigned)token);
+        }
+    };
     auto each = [&](int share, int turn, float least, auto&& what) {   // of a share's tokens those of the parts that reach `least`
-        const T* row = rows + share / a.per_beam * a.row_stride;
+        const T* row = rows + beam_of(share) * a.row_stride;
         const unsigned parts = __ballot_sync(0xffffffffu, s.parts[turn][warp][lane] >= least);
 #pragma unroll 1
-        for (int step = 0; step < steps; ++step) {
-            if (!(parts >> (step >> shift) & 1)) continue;
-            Raw8<T> x[kLines];
-            const int line = share % a.per_beam + step * kLines * a.per_beam;
-            read(row, line, x);
-#pragma unroll
-            for (int u = 0; u < kLines; ++u)
-                if (line + u * a.per_beam < a.lines)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float2 v = x[u].two(i / 2);
-                        what(i & 1 ? v.y : v.x, (unsigned)((line + u * a.per_beam) * kLine + lane * 8 + i));
-                    }
-        }
+        for (int step = 0; step < steps; ++step)
+            if (parts >> (step >> shift) & 1) few(row, part_of(share) + step * kLines * a.per_beam, least, what);
     };
     for (int share = me, turn = 0; share < shares; share += warps, ++turn) {
         if (!reaches(share)) continue;
-        const int b = share / a.per_beam;
+        const int b = beam_of(share);
         // a logit that may reach the bound, a little less than the one that does
         const double from = s.base[b] + (s.log_sum[b] + (bound - s.score[b]));
-        const float least = bound == -INFINITY ? -FLT_MAX : __double2float_rd(from - fabs(from) * 1e-12 - (fabs(s.base[b]) + fabs(s.score[b]) + fabs(s.log_sum[b])) * 1e-12);
-        each(share, turn, least, [&](float x, unsigned token) {
-            if (x >= least && total(b, x) >= bound) {
+        const float least = bound == -INFINITY ? -FLT_MAX : fmaxf(-FLT_MAX, __double2float_rd(from - fabs(from) * 1e-12 - (fabs(s.base[b]) + fabs(s.score[b]) + fabs(s.log_sum[b])) * 1e-12));   // never -inf: a token without a logit is none
+        auto take = [&](float x, unsigned token) {
+            if (total(b, x) >= bound) {
                 const int at = atomicAdd(&s.count, 1);
                 if (at < kFoundCap) s.found[at] = Found{ordered(total(b, x)), (unsigned)b * (unsigned)a.vocab + token, 0u};
             }
-        });
+        };
+        const float4 top = s.steps[turn][warp][lane];
+        if (__any_sync(0xffffffffu, top.z >= least)) { each(share, turn, least, take); continue; }
+        // no lane has more than two steps that reach it: every lane reads its own, all at once
+        const T* row = rows + b * a.row_stride;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+            const bool there = (i ? top.y : top.x) >= least;
+            if (!__any_sync(0xffffffffu, there)) break;
+            const unsigned which = __float_as_uint(top.w);
+            if (there) few(row, part_of(share) + (int)(i ? which >> 16 : which & 0xffffu) * kLines * a.per_beam, least, take);
+            __syncwarp();
+        }
     }
     __syncthreads();
     if (s.count > kFoundCap) {   // many totals alike: the k best of each share, one by one, and after each turn of the warps the block's k best
@@ -334,14 +415,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
         if (threadIdx.x == 0) s.count = 0;
         __syncthreads();
         for (int first = rank * kWarps, turn = 0; first < shares; first += warps, ++turn) {
-            const int share = first + warp, b = share / a.per_beam;
+            const int share = first + warp, b = beam_of(share);
             if (share < shares && reaches(share)) {
                 Found last{~0ull, 0u, 0u};
                 for (int i = 0; i < a.k; ++i) {
                     Found best{0ull, ~0u, 0u};
                     each(share, turn, -FLT_MAX, [&](float x, unsigned token) {
                         const Found f{ordered(total(b, x)), (unsigned)b * (unsigned)a.vocab + token, 0u};
-                        if (x != -INFINITY && (i == 0 || before(last, f)) && before(f, best)) best = f;
+                        if ((i == 0 || before(last, f)) && before(f, best)) best = f;
                     });
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) {
@@ -367,19 +448,32 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
     }
     cluster.sync();
     if (rank != 0) return;   // nobody looks into the other blocks any more
-    int n = 0;
-    for (int r = 0; r < blocks; ++r) n += s.counts[r];
-    for (int i = threadIdx.x; i < blocks * kMaxChosen; i += kThreads) {
-        const int r0 = i % blocks, j0 = i / blocks;
-        if (j0 >= s.counts[r0]) continue;
-        const Found mine = s.all[r0][j0];
+    if (warp == 0) {
+        const int mine = lane < blocks ? s.counts[lane] : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane <= blocks) s.first[lane] = upto - mine;
+    }
+    __syncthreads();
+    const int n = s.first[blocks];
+    for (int i = threadIdx.x; i < kMaxCluster * kMaxChosen; i += kThreads) {
+        const int r = i % kMaxCluster, j = i / kMaxCluster;
+        if (r < blocks && j < s.counts[r]) s.found[s.first[r] + j] = s.all[r][j];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const Found mine = s.found[i];
         int place = 0;
-        for (int r = 0; r < blocks; ++r)
-            for (int j = 0, end = s.counts[r]; j < end; ++j) place += before(s.all[r][j], mine);
+        for (int o = 0; o < n; ++o) place += before(s.found[o], mine);
         if (place < a.k) {
             const long long to = item * a.k + place;
-            a.parents[to] = (int)(mine.at / (unsigned)a.vocab);
-            a.tokens[to] = (int)(mine.at % (unsigned)a.vocab);
+            const unsigned parent = mine.at / (unsigned)a.vocab;
+            a.parents[to] = (int)parent;
+            a.tokens[to] = (int)(mine.at - parent * (unsigned)a.vocab);
             a.totals[to] = (float)from_ordered(mine.total);
         }
     }
@@ -399,9 +493,9 @@ psb_status select(SelectArgs a, int batch, int sms, cudaStream_t s) {
     while (blocks < kMaxCluster && (long long)batch * blocks * 2 <= 2 * sms && (long long)a.beams * a.lines >= (long long)blocks * kWarps * 2) blocks *= 2;
     const int warps = blocks * kWarps;
     a.per_beam = std::max(1, warps / a.beams);
-    // about 8 k groups for the bound
-    a.join = 1;
-    while (a.per_beam * a.beams / (2 * a.join) >= 8 * a.k) a.join *= 2;
+    a.by_beam = (unsigned)(((1ull << 32) + a.per_beam - 1) / a.per_beam);
+    a.groups = 32;
+    while (a.groups > 1 && a.per_beam * a.beams * a.groups > kMaxGroups) a.groups /= 2;
     const void* kernel = reinterpret_cast<const void*>(k_beam_select<T>);
     PSB_TRY(kernel_shared(kernel, sizeof(SelectShared)));
     if (blocks > 8) PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
