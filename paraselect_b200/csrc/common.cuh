@@ -146,6 +146,33 @@ __device__ __forceinline__ void mark_start(unsigned long long* mark) {
     if (mark && (blockIdx.x | blockIdx.y | blockIdx.z | threadIdx.x) == 0) asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(*mark));
 }
 
+// ---- device: two fp32 operations in one instruction ---------------------------------------------
+__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 halves(unsigned long long p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // ---- device: block-wide bitonic sort of n (power of two) keys in shared memory, ascending ---------
 template <typename K>
 __device__ __forceinline__ void block_bitonic_sort(K* s, int n) {

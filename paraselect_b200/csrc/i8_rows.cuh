@@ -1,0 +1,459 @@
+// Rows to 8-bit codes with one scale a row, plain or behind a residual addition and a root-mean-square norm:
+//   h = x + r,  u = h w,  code = rint(127 u / max|u|) (ties to even),  scale = max|u| / (127 rms),  rms = sqrt(mean h^2 + eps);
+// without the norm u = x and scale = max|x| / 127.  The norm's 1/rms is common to the row, so the codes do not depend on it.
+//
+// Codes are those of 64-bit arithmetic.  A code is first formed in fp32: with the norm u has a relative error of 2^-23 at most (one rounding in h, one
+// in the product), and so has the largest |u|; 127 / max|u| adds 2^-24, and the last product goes into a fused sum.  So t is off by less than
+// 127 * 5 * 2^-24 = 3.8e-5; without the norm by 127 * 2^-24 = 7.6e-6.  Only where t lies so near to a tie (one element in 12,500, or 50,000) it is
+// formed again in 64 bits from the row's own values, and for it the row's largest |u|, sought among the elements within 2^-21 of fp32's.  Rows whose
+// magnitudes leave fp32's safe range go through 64 bits altogether.
+//
+// Bound by memory: one pass over the row, which stays in registers between the reduction and the codes.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace psb {
+
+namespace {
+
+template <bool NORM> constexpr float kNearTie = 0.5f - (NORM ? 4e-5f : 1e-5f);
+constexpr float kNearTop = 1.0f - 1.0f / (1 << 21);
+constexpr float kSafeLow = 1e-30f, kSafeHigh = 1e30f;
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 16 bytes of neighbouring elements.
+template <typename T> struct Pack {
+    static constexpr int VEC = 16 / sizeof(T);
+    unsigned word[4];
+    // Elements [at, at + VEC) of a row of dim elements; with SHIFT some of them may be outside, which are left as they are.
+    template <bool SHIFT> __device__ __forceinline__ void read(const T* row, int at, int dim) {
+        if (!SHIFT || (at >= 0 && at + VEC <= dim)) set(*reinterpret_cast<const uint4*>(row + at));
+        else read_each(row, at, dim);
+    }
+    __device__ __forceinline__ void read_each(const T* row, int at, int dim) {   // wherever the row begins
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (at + e >= 0 && at + e < dim) put(e, row[at + e]);
+    }
+    __device__ __forceinline__ void put(int e, T v) {
+        if constexpr (sizeof(T) == 4) word[e] = *reinterpret_cast<const unsigned*>(&v);
+        else {
+            const unsigned u = *reinterpret_cast<const unsigned short*>(&v);
+            word[e >> 1] = e & 1 ? (word[e >> 1] & 0xffffu) | u << 16 : (word[e >> 1] & 0xffff0000u) | u;
+        }
+    }
+    // The same of the weight, whose first element lies at the beginning of a pack; AGAIN: a second time, rather than held in registers.
+    template <bool SHIFT, bool AGAIN = false> __device__ __forceinline__ void weigh(const T* w, int at, int dim, int shift) {
+        if constexpr (!SHIFT) {
+            if (AGAIN) load(w + at, word); else set(__ldg(reinterpret_cast<const uint4*>(w + at)));
+        } else weigh_shifted(w, at, dim, shift);
+    }
+    __device__ __forceinline__ void weigh_shifted(const T* w, int at, int dim, int shift) {
+        if (at < 0 || at + VEC > dim || (shift != 0 && at + shift + VEC > dim)) { read_each(w, at, dim); return; }
+        unsigned v[8];   // the packs that hold the first and the last of the elements
+        load(w + (at + shift - (shift ? VEC : 0)), v);
+        load(w + at + shift, v + 4);
+        // elements from VEC - shift of the two packs on, or all of the second
+        const int from = shift ? (VEC - shift) * (int)sizeof(T) : 16;
+        if (from & 8) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) v[i] = v[i + 2];
+        }
+        if (from & 16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = v[i + 4];
+        }
+        if (from & 4) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i) v[i] = v[i + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word[i] = sizeof(T) == 4 ? v[i] : __funnelshift_r(v[i], v[i + 1], (from & 2) * 8);
+    }
+    static __device__ __forceinline__ void load(const T* at, unsigned* to) {
+        asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(to[0]), "=r"(to[1]), "=r"(to[2]), "=r"(to[3]) : "l"(at));
+    }
+    __device__ __forceinline__ void zeros() { set(make_uint4(0, 0, 0, 0)); }
+    __device__ __forceinline__ void ones() {
+        constexpr unsigned kOnes = sizeof(T) == 4 ? 0x3f800000u : std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+        set(make_uint4(kOnes, kOnes, kOnes, kOnes));
+    }
+    __device__ __forceinline__ void set(uint4 v) { word[0] = v.x; word[1] = v.y; word[2] = v.z; word[3] = v.w; }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(word[e]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e & 1 ? word[e >> 1] & 0xffff0000u : word[e >> 1] << 16);
+        else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&word[e >> 1])); return e & 1 ? f.y : f.x; }
+    }
+    template <bool SHIFT> static __device__ __forceinline__ void write(T* row, int at, int dim, const unsigned long long* pairs) {
+        if (!SHIFT || (at >= 0 && at + VEC <= dim)) {
+            unsigned o[4];
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                const float2 v = halves(pairs[i]);
+                if constexpr (sizeof(T) == 4) { o[2 * i] = __float_as_uint(v.x); o[2 * i + 1] = __float_as_uint(v.y); }
+                else if constexpr (std::is_same<T, __nv_bfloat16>::value) { const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y); o[i] = *reinterpret_cast<const unsigned*>(&p); }
+                else { const __half2 p = __floats2half2_rn(v.x, v.y); o[i] = *reinterpret_cast<const unsigned*>(&p); }
+            }
+            *reinterpret_cast<uint4*>(row + at) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (at + e >= 0 && at + e < dim) { const float2 v = halves(pairs[e / 2]); row[at + e] = from_float<T>(e & 1 ? v.y : v.x); }
+        }
+    }
+};
+
+
+struct MaxOp { template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
+struct SumOp { template <typename V> __device__ V operator()(V a, V b) const { return a + b; } };
+
+template <int WIDTH, typename V, typename Op>
+__device__ __forceinline__ V lanes_reduce(V v, Op op) {
+#pragma unroll
+    for (int o = WIDTH >> 1; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+// Over the THREADS threads of a block.  `slots` holds a value a warp and is used once.
+template <int THREADS, typename V, typename Op>
+__device__ __forceinline__ V block_reduce(V v, V* slots, Op op) {
+    v = lanes_reduce<32>(v, op);
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return lanes_reduce<THREADS / 32>(slots[threadIdx.x & (THREADS / 32 - 1)], op);
+}
+
+// A magnitude's bits: their order as integers is that of the magnitudes, and a NaN's are above all.
+__device__ __forceinline__ unsigned long long magnitude(double v) { return (unsigned long long)__double_as_longlong(v) & 0x7fffffffffffffffull; }
+// The larger magnitude; NaN where either is.
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+struct LargerOp { __device__ float operator()(float a, float b) const { return larger(a, b); } };
+
+__device__ __forceinline__ signed char code64(double u, double top) { return (signed char)(int)rint(127.0 * u / top); }
+
+constexpr float kRint = 12582912.f;   // 1.5 * 2^23: a sum with it is rounded to whole numbers, which its lowest bits hold
+
+// Four codes' lowest bytes in one word.
+__device__ __forceinline__ unsigned four(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// The largest of a warp's values, NaN where there is one.
+__device__ __forceinline__ float warp_larger(float v) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in packs of 16 bytes.  What few elements need - 64 bits next to ties,
+// at the top, in rows out of fp32's range - is read again from memory, before the sum is written, by the 32 lanes of a warp for the one that found
+// it.  Code for it beside every element took five times the kernel's time, and a thread of its own for it half of the rest, the block waiting
+// (16,384 rows of 8,192 in bf16: 789 and 499 us).  fp32 arithmetic goes two elements an instruction: the kernel was bound by issue (239 us).
+//
+// SHIFT: rows that begin anywhere.  Packs are those of memory, so that the row begins in the middle of its first and ends in the middle of its last,
+// which are read and written element by element; the weight, whose packs lie otherwise, comes from two of them by a shift.  (7,000 rows of 8,191
+// in bf16 element by element: 317 us.)
+template <typename T, int kEach, int TPR, int MOST, bool NORM, bool SHIFT>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? (kEach == 32 ? (NORM ? 3 : 4) : (NORM ? 4 : 6)) : 1) k_i8_rows(RowArgs a) {
+    constexpr bool kBlock = TPR == 0;
+    constexpr int kPart = kBlock ? 32 : TPR;   // threads that exchange by shuffles
+    const int each_row = kBlock ? (int)blockDim.x : TPR;
+    using P = Pack<T>;
+    constexpr int VEC = P::VEC, NV = kEach / VEC;
+    static_assert(kEach <= 32, "a warp takes a lane's elements at once");
+    __shared__ float s_sum[MOST / 32], s_top[MOST / 32];
+    __shared__ unsigned long long s_top64;
+    __shared__ double s_sum64[MOST / 32];
+    const int lane = kBlock ? threadIdx.x : threadIdx.x % kPart, lane32 = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const long long row = kBlock ? blockIdx.x : (long long)blockIdx.x * (MOST / kPart) + threadIdx.x / kPart;
+    const bool live = row < a.n;
+    const T* w = NORM ? static_cast<const T*>(a.weight) : nullptr;
+    const int dim = live ? a.dim : 0;
+    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
+    // elements of the row's first pack that lie before the row
+    const int shift = SHIFT ? (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (VEC - 1) : 0;
+    auto begin = [&](int j) { return (j * each_row + lane) * VEC - shift; };   // of this thread's pack j in the row
+    if (kBlock && threadIdx.x == 0) s_top64 = 0;
+    unsigned long long h[kEach / 2];   // the row, or its sum with the residual, two elements each
+    float mine = 0.f, sum = 0.f;
+    {
+        const T* r = NORM && a.residual ? static_cast<const T*>(a.residual) + (live ? row : 0) * a.residual_stride : nullptr;
+        P px[NV], pr[NORM ? NV : 1], pw[NORM ? NV : 1];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            px[j].zeros();
+            if (NORM) { pr[j].zeros(); pw[j].ones(); }
+            const int at = begin(j);
+            if (at < dim) {
+                px[j].template read<SHIFT>(x, at, dim);
+                if (NORM && r) pr[j].template read<SHIFT>(r, at, dim);
+                if (NORM && w) pw[j].template weigh<SHIFT>(w, at, dim, shift);
+            }
+        }
+        unsigned long long sums = 0;
+#pragma unroll
+        for (int i = 0; i < kEach / 2; ++i) {
+            const int j = 2 * i / VEC, e = 2 * i % VEC;
+            h[i] = pair(px[j].get(e), px[j].get(e + 1));
+            float2 u = halves(h[i]);
+            if (NORM) {
+                if (r) h[i] = add2(h[i], pair(pr[j].get(e), pr[j].get(e + 1)));
+                sums = fma2(h[i], h[i], sums);
+                u = halves(mul2(h[i], pair(pw[j].get(e), pw[j].get(e + 1))));
+            }
+            mine = larger(larger(mine, u.x), u.y);
+        }
+        const float2 s = halves(sums);
+        sum = s.x + s.y;
+    }
+    float top32 = kPart == 32 ? warp_larger(mine) : lanes_reduce<kPart>(mine, LargerOp());
+    if (NORM) sum = lanes_reduce<kPart>(sum, SumOp());
+    if constexpr (kBlock) {
+        if (lane32 == 0) { s_top[threadIdx.x >> 5] = top32; s_sum[threadIdx.x >> 5] = sum; }
+        __syncthreads();
+        top32 = warp_larger(lane32 < warps ? s_top[lane32] : 0.f);
+        if (NORM) sum = lanes_reduce<32>(lane32 < warps ? s_sum[lane32] : 0.f, SumOp());
+    }
+    // (a NaN fails every comparison; a row without a norm has no sum to look at)
+    bool wild = !(top32 >= kSafeLow && top32 <= kSafeHigh) || (NORM && !(sum >= kSafeLow && sum <= kSafeHigh));
+    if (kBlock ? top32 == 0.f : __any_sync(0xffffffffu, top32 == 0.f)) {   // perhaps a row of zeros
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < kEach / 2; ++i) { const float2 v = halves(h[i]); some = some || v.x != 0.f || v.y != 0.f; }
+        some = kBlock ? __syncthreads_or(some) : lanes_reduce<kPart>((int)some, MaxOp());
+        if (top32 == 0.f && !some) wild = false;
+    }
+
+    // For each lane of the warp that needs it: f(lane, its row, element of the row, its value in 32 bits, its sum and value in 64), an element
+    // of that lane's for each of the 32 (an element < 0: none).
+    auto together = [&](bool need, auto&& f) {
+        __syncwarp();   // what f writes lies over what its lane wrote, what it reads under what that writes next
+        for (unsigned todo = __ballot_sync(0xffffffffu, need && live); todo; todo &= todo - 1) {
+            const int whose = __ffs(todo) - 1;
+            const long long of = __shfl_sync(0xffffffffu, row, whose);
+            const int l = kBlock ? (int)(threadIdx.x & ~31u) + whose : whose % kPart;
+            int i = (lane32 / VEC * each_row + l) * VEC + lane32 % VEC - (SHIFT ? __shfl_sync(0xffffffffu, shift, whose) : 0);
+            if (lane32 >= kEach || i >= a.dim) i = -1;
+            float v = 0.f;
+            double s64 = 0, v64 = 0;
+            if (i >= 0) {
+                const float x = to_float(static_cast<const T*>(a.x)[of * a.x_stride + i]);
+                const float r = NORM && a.residual ? to_float(static_cast<const T*>(a.residual)[of * a.residual_stride + i]) : 0.f;
+                const float by = NORM && w ? to_float(w[i]) : 1.f;
+                v = NORM ? (x + r) * by : x;
+                s64 = (double)x + (double)r;
+                v64 = s64 * (double)by;
+            }
+            f(whose, of, i, v, s64, v64);
+        }
+        __syncwarp();
+    };
+    const float inverse = top32 > 0 ? 127.f / top32 : 0.f;
+    signed char* out = a.codes + (live ? row : 0) * a.code_stride;
+    float off = 0.f;   // the furthest from a whole number
+    const unsigned long long by = pair(inverse, inverse), whole = pair(kRint, kRint), back = pair(-kRint, -kRint), minus = pair(-1.f, -1.f);
+    unsigned c[kEach];
+    {
+        P pw[NORM ? NV : 1];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (NORM) {
+                pw[j].ones();
+                const int at = begin(j);
+                if (w && at < dim) pw[j].template weigh<SHIFT, true>(w, at, dim, shift);
+            }
+#pragma unroll
+        for (int i = 0; i < kEach / 2; ++i) {
+            const int j = 2 * i / VEC, e = 2 * i % VEC;
+            unsigned long long u = h[i];
+            if (NORM) u = mul2(u, pair(pw[j].get(e), pw[j].get(e + 1)));
+            const unsigned long long m = fma2(u, by, whole), away = fma2(u, by, mul2(add2(m, back), minus));
+            const float2 code = halves(m), d = halves(away);
+            c[2 * i] = __float_as_uint(code.x);
+            c[2 * i + 1] = __float_as_uint(code.y);
+            off = fmaxf(fmaxf(off, fabsf(d.x)), fabsf(d.y));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int at = begin(j);
+        if (at >= dim) continue;
+        const unsigned* v = c + j * VEC;
+        if (!SHIFT || (at >= 0 && at + VEC <= dim && (reinterpret_cast<uintptr_t>(out + at) & (VEC - 1)) == 0)) {
+            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(out + at) = make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7]));
+            else *reinterpret_cast<unsigned*>(out + at) = four(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (at + e >= 0 && at + e < dim) out[at + e] = (signed char)v[e];
+        }
+    }
+    const bool unsure = wild || off > kNearTie<NORM>;
+    float scale = !(top32 > 0) ? 0.f : NORM ? top32 / (127.f * sqrtf(sum / (float)a.dim + a.eps)) : top32 / 127.f;
+    if (kBlock ? __syncthreads_or(unsure) : __any_sync(0xffffffffu, unsure)) {   // the row's largest magnitude in 64 bits, and the codes that need it
+        double top64 = top32;   // exact without a norm
+        if (NORM || (kBlock ? wild : __any_sync(0xffffffffu, wild))) {
+            unsigned long long t = 0;
+            const float near = top32 * kNearTop;
+            const bool of_row = kBlock ? true : lanes_reduce<kPart>((int)unsure, MaxOp()) != 0;   // (a part of a warp: the rows that need it)
+            together(wild || (NORM && of_row && mine >= near), [&](int whose, long long, int, float v, double, double v64) {
+                const bool all = __shfl_sync(0xffffffffu, (int)wild, whose);
+                const float least = __shfl_sync(0xffffffffu, near, whose);
+                const unsigned long long m = lanes_reduce<32>(all || fabsf(v) >= least ? magnitude(v64) : 0ull, MaxOp());
+                if (lane32 == whose) t = m;
+            });
+            if constexpr (!kBlock) t = lanes_reduce<kPart>(t, MaxOp());
+            else {
+                if (t) atomicMax(&s_top64, t);
+                __syncthreads();
+                t = s_top64;
+            }
+            if (NORM || wild) top64 = __longlong_as_double((long long)t);
+        }
+        bool dead = false;   // an infinity or a NaN: no codes, and a scale that says so
+        if (kBlock ? wild : __any_sync(0xffffffffu, wild)) {
+            double s = 0;
+            if (NORM) {
+                together(wild, [&](int whose, long long, int, float, double s64, double) {
+                    const double m = lanes_reduce<32>(s64 * s64, SumOp());
+                    if (lane32 == whose) s = m;
+                });
+                s = lanes_reduce<kPart>(s, SumOp());
+                if constexpr (kBlock) {
+                    if (lane32 == 0) s_sum64[threadIdx.x >> 5] = s;
+                    __syncthreads();
+                    s = lanes_reduce<32>(lane32 < warps ? s_sum64[lane32] : 0.0, SumOp());
+                }
+            }
+            if (wild) {
+                dead = !(top64 <= 1.7e308) || !(s <= 1.7e308);
+                scale = dead ? __int_as_float(0x7fffffff) : top64 > 0 ? (float)(top64 / (NORM ? 127.0 * sqrt(s / a.dim + (double)a.eps) : 127.0)) : 0.f;
+            }
+        }
+        together(unsure, [&](int whose, long long of, int i, float v, double, double v64) {
+            const bool all = __shfl_sync(0xffffffffu, (int)wild, whose), none = __shfl_sync(0xffffffffu, (int)dead, whose);
+            const double top = __shfl_sync(0xffffffffu, top64, whose);
+            const float by = __shfl_sync(0xffffffffu, inverse, whose), m = fmaf(v, by, kRint);
+            if (i >= 0 && (all || fabsf(fmaf(v, by, kRint - m)) > kNearTie<NORM>)) a.codes[of * a.code_stride + i] = none || top == 0 ? (signed char)0 : code64(v64, top);
+        });
+    }
+    if (NORM && a.sum) {
+        T* to = static_cast<T*>(a.sum) + (live ? row : 0) * a.sum_stride;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (begin(j) < dim) P::template write<SHIFT>(to, begin(j), dim, h + j * (VEC / 2));
+    }
+    if (live && lane == 0) a.scales[row] = scale;
+}
+
+// Rows too long for registers, or whose arrays begin at places that differ within a pack: a block a row, element by element, read again for the codes
+// (from L2, as a rule).  Each thread writes only
+// elements it has read itself, so the sum may lie over the rows or the residual.
+template <typename T, bool NORM, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_i8_rows_any(RowArgs a) {
+    __shared__ double s_sum64[32];
+    __shared__ unsigned long long s_top64[32];
+    const long long row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* r = NORM && a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+    const T* w = NORM ? static_cast<const T*>(a.weight) : nullptr;
+    auto sum_of = [&](int i) { return (double)to_float(x[i]) + (r ? (double)to_float(r[i]) : 0.0); };
+    double sum = 0;
+    unsigned long long t = 0;
+    for (int i = threadIdx.x; i < a.dim; i += THREADS) {
+        const double h = sum_of(i);
+        if (NORM) sum = fma(h, h, sum);
+        t = max(t, magnitude(w ? h * (double)to_float(w[i]) : h));
+    }
+    const double top = __longlong_as_double((long long)block_reduce<THREADS>(t, s_top64, MaxOp()));
+    const double mean = NORM ? block_reduce<THREADS>(sum, s_sum64, SumOp()) / a.dim : 0;
+    const bool dead = !(top <= 1.7e308) || !(mean <= 1.7e308);
+    if (threadIdx.x == 0) {
+        const double by = NORM ? 127.0 * sqrt(mean + (double)a.eps) : 127.0;
+        a.scales[row] = dead ? __int_as_float(0x7fffffff) : top > 0 ? (float)(top / by) : 0.f;
+    }
+    for (int i = threadIdx.x; i < a.dim; i += THREADS) {
+        const double h = sum_of(i);
+        const float h32 = r ? to_float(x[i]) + to_float(r[i]) : to_float(x[i]);
+        a.codes[row * a.code_stride + i] = dead || top == 0 ? 0 : code64(w ? h * (double)to_float(w[i]) : h, top);
+        if (NORM && a.sum) static_cast<T*>(a.sum)[row * a.sum_stride + i] = from_float<T>(h32);
+    }
+}
+
+template <typename T, int kEach, int TPR, int MOST, bool NORM, bool SHIFT>
+psb_status start(const RowArgs& a, int threads, cudaStream_t s) {
+    const long long rows = TPR ? MOST / (TPR ? TPR : 1) : 1, blocks = (a.n + rows - 1) / rows;
+    k_i8_rows<T, kEach, TPR, MOST, NORM, SHIFT><<<(unsigned)blocks, TPR ? MOST : threads, 0, s>>>(a);
+    PSB_LAUNCH_CHECK();
+    count_launch();
+    return PSB_OK;
+}
+
+// As few threads a row as hold it in registers, 32 elements of two bytes or 16 of four each, since what a thread does once a row is then shared among
+// most (16,384 rows of 8,192 in bf16: 172 us with 32 elements, 212 with 16); more of them, with 16 elements, where rows are too few to fill the
+// GPU (one row of 4,096: 3.0 us, with 32 3.6).
+template <typename T, bool NORM, bool SHIFT>
+psb_status by_length(const RowArgs& a, int sms, cudaStream_t s) {
+    constexpr int VEC = Pack<T>::VEC, kMost = VEC == 8 ? 32 : 16;
+    const int span = a.dim + (SHIFT ? VEC - 1 : 0);
+    auto warps = [&](int each) { return ((span + each - 1) / each + 31) / 32 * 32; };   // threads, in whole warps
+    if (span > 512 && a.n * (long long)warps(kMost) < 1024ll * sms && warps(16) <= 1024) {
+        int threads = warps(16);
+        while (threads <= 512 && threads < warps(VEC) && a.n * (long long)threads < 1024ll * sms) threads *= 2;
+        return start<T, 16, 0, 1024, NORM, SHIFT>(a, std::min(threads, warps(VEC)), s);
+    }
+    if (span <= 4 * 16) return start<T, 16, 4, 256, NORM, SHIFT>(a, 0, s);
+    if (span <= 4 * kMost) return start<T, kMost, 4, 256, NORM, SHIFT>(a, 0, s);
+    if (span <= 8 * kMost) return start<T, kMost, 8, 256, NORM, SHIFT>(a, 0, s);
+    if (span <= 16 * kMost) return start<T, kMost, 16, 256, NORM, SHIFT>(a, 0, s);
+    if (span <= 32 * kMost) return start<T, kMost, 32, 256, NORM, SHIFT>(a, 0, s);
+    if (span <= 256 * kMost) return start<T, kMost, 0, 256, NORM, SHIFT>(a, warps(kMost), s);
+    if (span <= 512 * kMost) return start<T, kMost, 0, 512, NORM, SHIFT>(a, warps(kMost), s);
+    return start<T, kMost, 0, 1024, NORM, SHIFT>(a, warps(kMost), s);
+}
+
+template <typename T, bool NORM>
+psb_status by_layout(const RowArgs& a, int sms, cudaStream_t s) {
+    constexpr int VEC = Pack<T>::VEC;
+    auto place = [](const void* p, long long each) { return (int)(reinterpret_cast<uintptr_t>(p) / each & (VEC - 1)); };   // within a pack
+    const int e = sizeof(T), at = place(a.x, e), step = (int)(a.x_stride & (VEC - 1));
+    // the rows' arrays begin at the same place of a pack in every row
+    auto as_rows = [&](const void* p, long long stride) { return !p || (place(p, e) == at && (int)(stride & (VEC - 1)) == step); };
+    const bool packs = as_rows(a.residual, a.residual_stride) && as_rows(a.sum, a.sum_stride) && place(a.weight, e) == 0;
+    if (packs && a.dim + VEC - 1 <= 1024 * (VEC == 8 ? 32 : 16)) {
+        const bool plain = at == 0 && step == 0 && a.dim % VEC == 0 && place(a.codes, 1) == 0 && (a.code_stride & (VEC - 1)) == 0;
+        return plain ? by_length<T, NORM, false>(a, sms, s) : by_length<T, NORM, true>(a, sms, s);
+    }
+    if (a.dim <= 4096) k_i8_rows_any<T, NORM, 128><<<(unsigned)a.n, 128, 0, s>>>(a);
+    else k_i8_rows_any<T, NORM, 1024><<<(unsigned)a.n, 1024, 0, s>>>(a);
+    PSB_LAUNCH_CHECK();
+    count_launch();
+    return PSB_OK;
+}
+
+}  // namespace
+
+// What an element type's file defines.
+template <typename T> psb_status launch_i8_rows(const RowArgs& a, bool norm, int sms, cudaStream_t s) {
+    return norm ? by_layout<T, true>(a, sms, s) : by_layout<T, false>(a, sms, s);
+}
+
+}  // namespace psb

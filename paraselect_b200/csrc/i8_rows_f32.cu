@@ -1,0 +1,5 @@
+#include "i8_rows.cuh"
+
+namespace psb {
+psb_status i8_rows_f32(const RowArgs& a, bool norm, int sms, cudaStream_t s) { return launch_i8_rows<float>(a, norm, sms, s); }
+}  // namespace psb

@@ -414,6 +414,22 @@ psb_status launch_gen_mixture(const float* d_centres, const long long* d_offsets
 psb_status launch_gen_normal(uint64_t seed, long long first, long long n, float scale, float* d_out,
                              cudaStream_t s);
 
+// ---- rows of 8-bit codes (i8_rows.cuh; a file for each element type) --------------------------------------------
+struct RowArgs {
+    const void* x;
+    const void* residual;   // may be null
+    const void* weight;     // may be null (ones)
+    void* sum;              // may be null; may be x or residual
+    signed char* codes;
+    float* scales;
+    long long n, x_stride, residual_stride, sum_stride, code_stride;
+    int dim;
+    float eps;
+};
+psb_status i8_rows_f32(const RowArgs& a, bool norm, int sms, cudaStream_t s);
+psb_status i8_rows_f16(const RowArgs& a, bool norm, int sms, cudaStream_t s);
+psb_status i8_rows_bf16(const RowArgs& a, bool norm, int sms, cudaStream_t s);
+
 // What the group layer (group.cu) needs to know of a session.
 struct SessionShape {
     int dim = 0, m = 0, k = 0, nlist = 0, n_rerank = 0, exact_elem = 0, device = 0;
