@@ -40,12 +40,14 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 template <typename T> struct Pack {
     static constexpr int VEC = 16 / sizeof(T);
     unsigned word[4];
-    // Elements [at, at + VEC) of a row of dim elements; with SHIFT some of them may be outside, which are left as they are.
-    template <bool SHIFT> __device__ __forceinline__ void read(const T* row, int at, int dim) {
-        if (!SHIFT || (at >= 0 && at + VEC <= dim)) set(*reinterpret_cast<const uint4*>(row + at));
-        else read_each(row, at, dim);
+    // Elements [at, at + VEC) of a row, which begin a pack of memory.
+    __device__ __forceinline__ void read(const T* row, int at) { set(*reinterpret_cast<const uint4*>(row + at)); }
+    // A second time, rather than held in registers.
+    __device__ __forceinline__ void read_again(const T* row, int at) {
+        asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(word[0]), "=r"(word[1]), "=r"(word[2]), "=r"(word[3]) : "l"(row + at));
     }
-    __device__ __forceinline__ void read_each(const T* row, int at, int dim) {   // wherever the row begins
+    // Those of them that a row of dim elements has, wherever it begins; the others are left as they are.
+    __device__ __forceinline__ void read_each(const T* row, int at, int dim) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
             if (at + e >= 0 && at + e < dim) put(e, row[at + e]);
@@ -56,37 +58,6 @@ template <typename T> struct Pack {
             const unsigned u = *reinterpret_cast<const unsigned short*>(&v);
             word[e >> 1] = e & 1 ? (word[e >> 1] & 0xffffu) | u << 16 : (word[e >> 1] & 0xffff0000u) | u;
         }
-    }
-    // The same of the weight, whose first element lies at the beginning of a pack; AGAIN: a second time, rather than held in registers.
-    template <bool SHIFT, bool AGAIN = false> __device__ __forceinline__ void weigh(const T* w, int at, int dim, int shift) {
-        if constexpr (!SHIFT) {
-            if (AGAIN) load(w + at, word); else set(__ldg(reinterpret_cast<const uint4*>(w + at)));
-        } else weigh_shifted(w, at, dim, shift);
-    }
-    __device__ __forceinline__ void weigh_shifted(const T* w, int at, int dim, int shift) {
-        if (at < 0 || at + VEC > dim || (shift != 0 && at + shift + VEC > dim)) { read_each(w, at, dim); return; }
-        unsigned v[8];   // the packs that hold the first and the last of the elements
-        load(w + (at + shift - (shift ? VEC : 0)), v);
-        load(w + at + shift, v + 4);
-        // elements from VEC - shift of the two packs on, or all of the second
-        const int from = shift ? (VEC - shift) * (int)sizeof(T) : 16;
-        if (from & 8) {
-#pragma unroll
-            for (int i = 0; i < 6; ++i) v[i] = v[i + 2];
-        }
-        if (from & 16) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = v[i + 4];
-        }
-        if (from & 4) {
-#pragma unroll
-            for (int i = 0; i < 5; ++i) v[i] = v[i + 1];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) word[i] = sizeof(T) == 4 ? v[i] : __funnelshift_r(v[i], v[i + 1], (from & 2) * 8);
-    }
-    static __device__ __forceinline__ void load(const T* at, unsigned* to) {
-        asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(to[0]), "=r"(to[1]), "=r"(to[2]), "=r"(to[3]) : "l"(at));
     }
     __device__ __forceinline__ void zeros() { set(make_uint4(0, 0, 0, 0)); }
     __device__ __forceinline__ void ones() {
@@ -163,38 +134,57 @@ __device__ __forceinline__ float warp_larger(float v) {
     return r;
 }
 
+// Blocks of MOST threads that an SM's registers shall hold.
+template <int kEach, int MOST, bool NORM> constexpr int blocks_of() { return MOST == 256 ? (kEach == 32 ? (NORM ? 3 : 4) : (NORM ? 4 : 6)) : MOST == 288 ? 2 : 1; }
+
 // One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in packs of 16 bytes.  What few elements need - 64 bits next to ties,
 // at the top, in rows out of fp32's range - is read again from memory, before the sum is written, by the 32 lanes of a warp for the one that found
 // it.  Code for it beside every element took five times the kernel's time, and a thread of its own for it half of the rest, the block waiting
 // (16,384 rows of 8,192 in bf16: 789 and 499 us).  fp32 arithmetic goes two elements an instruction: the kernel was bound by issue (239 us).
 //
-// SHIFT: rows that begin anywhere.  Packs are those of memory, so that the row begins in the middle of its first and ends in the middle of its last,
-// which are read and written element by element; the weight, whose packs lie otherwise, comes from two of them by a shift.  (7,000 rows of 8,191
-// in bf16 element by element: 317 us.)
+// SHIFT: rows that begin anywhere.  Packs are those of memory, so that the row begins in the middle of its first and ends in the middle of its last, at
+// the same places in all rows of a block.  Those two are read and written element by element.  With a weight, whose packs lie otherwise, a block takes
+// every G-th row, G a multiple of a pack's elements, so that the weight is laid out once, in shared memory; the two packs are then read whole, but for
+// the first row's first and the last row's last, and what belongs to the neighbouring rows is put to zero.  (7,000 rows of 8,191 in bf16 element by
+// element: 317 us, with the weight's packs shifted anew for each row 273, so 127.  Rows that begin at packs lose by keeping the weight: 74 us and 82.)
 template <typename T, int kEach, int TPR, int MOST, bool NORM, bool SHIFT>
-__global__ void __launch_bounds__(MOST, MOST == 256 ? (kEach == 32 ? (NORM ? 3 : 4) : (NORM ? 4 : 6)) : 1) k_i8_rows(RowArgs a) {
+__global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_rows(RowArgs a) {
     constexpr bool kBlock = TPR == 0;
     constexpr int kPart = kBlock ? 32 : TPR;   // threads that exchange by shuffles
     const int each_row = kBlock ? (int)blockDim.x : TPR;
     using P = Pack<T>;
     constexpr int VEC = P::VEC, NV = kEach / VEC;
+    constexpr bool kKeep = NORM && SHIFT;
     static_assert(kEach <= 32, "a warp takes a lane's elements at once");
     __shared__ float s_sum[MOST / 32], s_top[MOST / 32];
-    __shared__ unsigned long long s_top64;
+    __shared__ unsigned long long s_tops64[2];   // of this row and the next
     __shared__ double s_sum64[MOST / 32];
     const int lane = kBlock ? threadIdx.x : threadIdx.x % kPart, lane32 = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const long long row = kBlock ? blockIdx.x : (long long)blockIdx.x * (MOST / kPart) + threadIdx.x / kPart;
-    const bool live = row < a.n;
     const T* w = NORM ? static_cast<const T*>(a.weight) : nullptr;
-    const int dim = live ? a.dim : 0;
-    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
-    // elements of the row's first pack that lie before the row
-    const int shift = SHIFT ? (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (VEC - 1) : 0;
+    const long long first = kBlock ? blockIdx.x : (long long)blockIdx.x * (MOST / kPart) + threadIdx.x / kPart, step = kBlock ? gridDim.x : (long long)gridDim.x * (MOST / kPart);
+    // elements of a row's first pack that lie before the row
+    const int shift = SHIFT ? (int)(reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + first * a.x_stride) / sizeof(T)) & (VEC - 1) : 0;
     auto begin = [&](int j) { return (j * each_row + lane) * VEC - shift; };   // of this thread's pack j in the row
-    if (kBlock && threadIdx.x == 0) s_top64 = 0;
+    if (kBlock && threadIdx.x == 0) s_tops64[0] = 0;
+    extern __shared__ uint4 s_weight[];   // kKeep: the weight's packs of each thread
+    if (kKeep)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            P p;
+            p.ones();
+            if (w && begin(j) < a.dim) p.read_each(w, begin(j), a.dim);
+            s_weight[j * blockDim.x + threadIdx.x] = make_uint4(p.word[0], p.word[1], p.word[2], p.word[3]);
+        }
+    int turn = 0;
+    long long row = first;
+    // (a part of a warp whose rows have ended stays for the others)
+    do {
+    const bool live = row < a.n;
+    const int dim = live ? a.dim : 0;
     unsigned long long h[kEach / 2];   // the row, or its sum with the residual, two elements each
     float mine = 0.f, sum = 0.f;
     {
+        const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
         const T* r = NORM && a.residual ? static_cast<const T*>(a.residual) + (live ? row : 0) * a.residual_stride : nullptr;
         P px[NV], pr[NORM ? NV : 1], pw[NORM ? NV : 1];
 #pragma unroll
@@ -203,23 +193,35 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? (kEach == 32 ? (NORM ? 3 :
             if (NORM) { pr[j].zeros(); pw[j].ones(); }
             const int at = begin(j);
             if (at < dim) {
-                px[j].template read<SHIFT>(x, at, dim);
-                if (NORM && r) pr[j].template read<SHIFT>(r, at, dim);
-                if (NORM && w) pw[j].template weigh<SHIFT>(w, at, dim, shift);
+                if (NORM && !kKeep && w) pw[j].read(w, at);
+                if (!SHIFT || (at >= 0 && at + VEC <= dim) || (kKeep && (row > 0 || at >= 0) && (row < a.n - 1 || at + VEC <= dim))) {
+                    px[j].read(x, at);
+                    if (NORM && r) pr[j].read(r, at);
+                } else {
+                    px[j].read_each(x, at, dim);
+                    if (NORM && r) pr[j].read_each(r, at, dim);
+                }
             }
         }
         unsigned long long sums = 0;
 #pragma unroll
-        for (int i = 0; i < kEach / 2; ++i) {
-            const int j = 2 * i / VEC, e = 2 * i % VEC;
-            h[i] = pair(px[j].get(e), px[j].get(e + 1));
-            float2 u = halves(h[i]);
-            if (NORM) {
-                if (r) h[i] = add2(h[i], pair(pr[j].get(e), pr[j].get(e + 1)));
-                sums = fma2(h[i], h[i], sums);
-                u = halves(mul2(h[i], pair(pw[j].get(e), pw[j].get(e + 1))));
+        for (int j = 0; j < NV; ++j) {
+            const int at = begin(j);
+            const bool edge = kKeep && (at < 0 || at + VEC > dim);
+            if (kKeep) pw[j].set(s_weight[j * blockDim.x + threadIdx.x]);
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+                const int i = (j * VEC + e) / 2;
+                h[i] = pair(px[j].get(e), px[j].get(e + 1));
+                if (NORM && r) h[i] = add2(h[i], pair(pr[j].get(e), pr[j].get(e + 1)));
+                if (edge) {
+                    const float2 v = halves(h[i]);
+                    h[i] = pair((unsigned)(at + e) < (unsigned)dim ? v.x : 0.f, (unsigned)(at + e + 1) < (unsigned)dim ? v.y : 0.f);
+                }
+                if (NORM) sums = fma2(h[i], h[i], sums);
+                const float2 u = halves(NORM ? mul2(h[i], pair(pw[j].get(e), pw[j].get(e + 1))) : h[i]);
+                mine = larger(larger(mine, u.x), u.y);
             }
-            mine = larger(larger(mine, u.x), u.y);
         }
         const float2 s = halves(sums);
         sum = s.x + s.y;
@@ -229,6 +231,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? (kEach == 32 ? (NORM ? 3 :
     if constexpr (kBlock) {
         if (lane32 == 0) { s_top[threadIdx.x >> 5] = top32; s_sum[threadIdx.x >> 5] = sum; }
         __syncthreads();
+        if (threadIdx.x == 0) s_tops64[(turn + 1) & 1] = 0;
         top32 = warp_larger(lane32 < warps ? s_top[lane32] : 0.f);
         if (NORM) sum = lanes_reduce<32>(lane32 < warps ? s_sum[lane32] : 0.f, SumOp());
     }
@@ -271,20 +274,17 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? (kEach == 32 ? (NORM ? 3 :
     float off = 0.f;   // the furthest from a whole number
     const unsigned long long by = pair(inverse, inverse), whole = pair(kRint, kRint), back = pair(-kRint, -kRint), minus = pair(-1.f, -1.f);
     unsigned c[kEach];
-    {
-        P pw[NORM ? NV : 1];
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (NORM) {
-                pw[j].ones();
-                const int at = begin(j);
-                if (w && at < dim) pw[j].template weigh<SHIFT, true>(w, at, dim, shift);
-            }
+    for (int j = 0; j < NV; ++j) {
+        P pw;
+        if (NORM) pw.ones();
+        if (kKeep) pw.set(s_weight[j * blockDim.x + threadIdx.x]);
+        else if (NORM && w && begin(j) < dim) pw.read_again(w, begin(j));
 #pragma unroll
-        for (int i = 0; i < kEach / 2; ++i) {
-            const int j = 2 * i / VEC, e = 2 * i % VEC;
+        for (int e = 0; e < VEC; e += 2) {
+            const int i = (j * VEC + e) / 2;
             unsigned long long u = h[i];
-            if (NORM) u = mul2(u, pair(pw[j].get(e), pw[j].get(e + 1)));
+            if (NORM) u = mul2(u, pair(pw.get(e), pw.get(e + 1)));
             const unsigned long long m = fma2(u, by, whole), away = fma2(u, by, mul2(add2(m, back), minus));
             const float2 code = halves(m), d = halves(away);
             c[2 * i] = __float_as_uint(code.x);
@@ -322,9 +322,9 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? (kEach == 32 ? (NORM ? 3 :
             });
             if constexpr (!kBlock) t = lanes_reduce<kPart>(t, MaxOp());
             else {
-                if (t) atomicMax(&s_top64, t);
+                if (t) atomicMax(&s_tops64[turn & 1], t);
                 __syncthreads();
-                t = s_top64;
+                t = s_tops64[turn & 1];
             }
             if (NORM || wild) top64 = __longlong_as_double((long long)t);
         }
@@ -362,6 +362,9 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? (kEach == 32 ? (NORM ? 3 :
             if (begin(j) < dim) P::template write<SHIFT>(to, begin(j), dim, h + j * (VEC / 2));
     }
     if (live && lane == 0) a.scales[row] = scale;
+    row += step;
+    ++turn;
+    } while (kKeep && (kBlock ? row < a.n : __any_sync(0xffffffffu, row < a.n)));
 }
 
 // Rows too long for registers, or whose arrays begin at places that differ within a pack: a block a row, element by element, read again for the codes
@@ -399,9 +402,18 @@ __global__ void __launch_bounds__(THREADS) k_i8_rows_any(RowArgs a) {
 }
 
 template <typename T, int kEach, int TPR, int MOST, bool NORM, bool SHIFT>
-psb_status start(const RowArgs& a, int threads, cudaStream_t s) {
+psb_status start(const RowArgs& a, int threads, int sms, cudaStream_t s) {
+    if (TPR) threads = MOST;
     const long long rows = TPR ? MOST / (TPR ? TPR : 1) : 1, blocks = (a.n + rows - 1) / rows;
-    k_i8_rows<T, kEach, TPR, MOST, NORM, SHIFT><<<(unsigned)blocks, TPR ? MOST : threads, 0, s>>>(a);
+    long long grid = blocks;
+    if (NORM && SHIFT) {   // as many blocks as fit, of as many rows each as the others, a multiple of a pack's elements
+        const long long fit = (long long)sms * std::max(1, blocks_of<kEach, MOST, NORM>() * MOST / threads), turns = (blocks + fit - 1) / fit;
+        grid = (blocks + turns - 1) / turns;
+        if (grid < blocks) grid = std::min(blocks, std::max(8ll, std::min((grid + 7) / 8 * 8, fit / 8 * 8)));
+    }
+    const size_t weight = NORM && SHIFT ? (size_t)threads * kEach * sizeof(T) : 0;
+    if (weight > 48 * 1024) PSB_TRY(kernel_shared(reinterpret_cast<const void*>(k_i8_rows<T, kEach, TPR, MOST, NORM, SHIFT>), weight));
+    k_i8_rows<T, kEach, TPR, MOST, NORM, SHIFT><<<(unsigned)grid, threads, weight, s>>>(a);
     PSB_LAUNCH_CHECK();
     count_launch();
     return PSB_OK;
@@ -418,16 +430,17 @@ psb_status by_length(const RowArgs& a, int sms, cudaStream_t s) {
     if (span > 512 && a.n * (long long)warps(kMost) < 1024ll * sms && warps(16) <= 1024) {
         int threads = warps(16);
         while (threads <= 512 && threads < warps(VEC) && a.n * (long long)threads < 1024ll * sms) threads *= 2;
-        return start<T, 16, 0, 1024, NORM, SHIFT>(a, std::min(threads, warps(VEC)), s);
+        return start<T, 16, 0, 1024, NORM, SHIFT>(a, std::min(threads, warps(VEC)), sms, s);
     }
-    if (span <= 4 * 16) return start<T, 16, 4, 256, NORM, SHIFT>(a, 0, s);
-    if (span <= 4 * kMost) return start<T, kMost, 4, 256, NORM, SHIFT>(a, 0, s);
-    if (span <= 8 * kMost) return start<T, kMost, 8, 256, NORM, SHIFT>(a, 0, s);
-    if (span <= 16 * kMost) return start<T, kMost, 16, 256, NORM, SHIFT>(a, 0, s);
-    if (span <= 32 * kMost) return start<T, kMost, 32, 256, NORM, SHIFT>(a, 0, s);
-    if (span <= 256 * kMost) return start<T, kMost, 0, 256, NORM, SHIFT>(a, warps(kMost), s);
-    if (span <= 512 * kMost) return start<T, kMost, 0, 512, NORM, SHIFT>(a, warps(kMost), s);
-    return start<T, kMost, 0, 1024, NORM, SHIFT>(a, warps(kMost), s);
+    if (span <= 4 * 16) return start<T, 16, 4, 256, NORM, SHIFT>(a, 0, sms, s);
+    if (span <= 4 * kMost) return start<T, kMost, 4, 256, NORM, SHIFT>(a, 0, sms, s);
+    if (span <= 8 * kMost) return start<T, kMost, 8, 256, NORM, SHIFT>(a, 0, sms, s);
+    if (span <= 16 * kMost) return start<T, kMost, 16, 256, NORM, SHIFT>(a, 0, sms, s);
+    if (span <= 32 * kMost) return start<T, kMost, 32, 256, NORM, SHIFT>(a, 0, sms, s);
+    if (span <= 256 * kMost) return start<T, kMost, 0, 256, NORM, SHIFT>(a, warps(kMost), sms, s);
+    if (span <= 288 * kMost) return start<T, kMost, 0, 288, NORM, SHIFT>(a, warps(kMost), sms, s);
+    if (span <= 512 * kMost) return start<T, kMost, 0, 512, NORM, SHIFT>(a, warps(kMost), sms, s);
+    return start<T, kMost, 0, 1024, NORM, SHIFT>(a, warps(kMost), sms, s);
 }
 
 template <typename T, bool NORM>
