@@ -4,7 +4,7 @@
 //
 // The rows of w (channels, stored rows) take the tensor cores' M side, 128 to a block, and the rows of x (tokens, queries) the N side, up to
 // 256: a thread of the epilogue then holds one channel for all tokens, a warp 32 neighbouring channels, and its stores of a token's outputs
-// lie side by side without a pass through shared memory.  One token is the same kernel with 16 columns, bound by the reading of w.
+// lie side by side without a pass through shared memory.
 //
 // k runs through shared memory in slabs of 128 codes (one 128-byte swizzle row), loaded by TMA into a ring; codes behind the end of a row and
 // rows behind the last are the TMA's zeros.  Few tiles are split along k over a cluster of up to 8 blocks, which hold their partial sums in
@@ -35,8 +35,10 @@ constexpr int kMaxTokens = 256;            // rows of x a tile
 constexpr int kEpilogue = 8;               // epilogue warps: two to each quarter of the tensor memory's lanes
 constexpr int kThreads = 32 * kEpilogue + 64;   // one warp loads, one issues products
 constexpr int kMaxStages = 12;
+constexpr int kMaxParts = 8;               // blocks that share a tile
 constexpr int kRing = 200 * 1024;
 constexpr int kWaitPolls = 1 << 22;
+constexpr long long kAllTiles = 0x7fffffffffffffffll;
 
 struct MatmulArgs {
     const signed char* x;
@@ -91,6 +93,38 @@ __device__ int dot_codes(const signed char* a, const signed char* b, int k) {
     for (; i + 4 <= k; i += 4) s = __dp4a(*reinterpret_cast<const int*>(a + i), *reinterpret_cast<const int*>(b + i), s);
     for (; i < k; ++i) s += (int)a[i] * (int)b[i];
     return s;
+}
+
+// An epilogue warp's half of the columns of a tile, 32 channels: channel c in this thread, tokens from t0.  Every epilogue warp of the block calls it.
+// `scales`: the other of the two buffers still serves slower warps' last tile.
+template <typename T>
+__device__ __forceinline__ void store_tile(const MatmulArgs& a, float* scales, uint32_t from, int c, int t0, int warp, int lane) {
+    const int half = warp >> 2, i0 = warp * 32 + lane;
+    if (i0 < a.tokens) scales[i0] = t0 + i0 < a.m ? __ldg(a.x_scales + t0 + i0) : 0.f;
+    const bool here = c < a.n;
+    const float ws = here ? __ldg(a.w_scales + c) : 0.f;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogue) : "memory");
+    T* out = static_cast<T*>(a.out) + (long long)(t0 + half * 16) * a.out_stride + c;
+    const int live = min(a.tokens, a.m - t0);
+    for (int t = half * 16; t < live; t += 32, out += 32 * a.out_stride) {
+        uint32_t v[16];
+        tmem_ld16(from + t, v);
+        float by[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(by + i) = *reinterpret_cast<const float4*>(scales + t + i);
+        tc::tmem_ld_wait();
+        if (here) {
+            T* to = out;
+            if (t + 16 <= live) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i, to += a.out_stride) *to = rounded<T>((float)(int)v[i] * by[i] * ws);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i, to += a.out_stride)
+                    if (t + i < live) *to = rounded<T>((float)(int)v[i] * by[i] * ws);
+            }
+        }
+    }
 }
 
 // SPLIT: the blocks of a cluster share a tile, each with its share of the slabs.  Otherwise a block takes every gridDim.x-th tile, its
@@ -202,33 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
                     for (int i = 0; i < 16; ++i) partial[(t + i) * kChannels + c] = (int)v[i];
                 }
             } else {
-                float* scales = s_scales[count & 1];   // the other half still serves slower warps' last tile
-                const int i0 = warp * 32 + lane;
-                if (i0 < a.tokens) scales[i0] = t0 + i0 < a.m ? __ldg(a.x_scales + t0 + i0) : 0.f;
-                const bool here = c0 + c < a.n;
-                const float ws = here ? __ldg(a.w_scales + c0 + c) : 0.f;
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogue) : "memory");
-                T* out = static_cast<T*>(a.out) + (long long)(t0 + half * 16) * a.out_stride + c0 + c;
-                const int live = min(a.tokens, a.m - t0);
-                for (int t = half * 16; t < live; t += 32, out += 32 * a.out_stride) {
-                    uint32_t v[16];
-                    tmem_ld16(from + t, v);
-                    float by[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(by + i) = *reinterpret_cast<const float4*>(scales + t + i);
-                    tc::tmem_ld_wait();
-                    if (here) {
-                        T* to = out;
-                        if (t + 16 <= live) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i, to += a.out_stride) *to = rounded<T>((float)(int)v[i] * by[i] * ws);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i, to += a.out_stride)
-                                if (t + i < live) *to = rounded<T>((float)(int)v[i] * by[i] * ws);
-                        }
-                    }
-                }
+                store_tile<T>(a, s_scales[count & 1], from, c0 + c, t0, warp, lane);
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&drained[buf])) : "memory");
@@ -250,22 +258,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
         // four channels a thread: 32 threads a token
         constexpr int kWarps = kThreads / 32;
         const int c4 = (threadIdx.x & 31) * 4;
+        float ws[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ws[e] = c0 + c4 + e < a.n ? __ldg(a.w_scales + c0 + c4 + e) : 0.f;
         for (int t = part * kWarps + warp; t < a.tokens && t0 + t < a.m; t += kWarps * parts) {
+            const float by = __ldg(a.x_scales + t0 + t);
             int s[4] = {0, 0, 0, 0};
             if (!lost) {
-                for (int p = 0; p < parts; ++p) {
-                    const int4 v = *reinterpret_cast<const int4*>(cluster.map_shared_rank(partial, p) + t * kChannels + c4);
-                    s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
-                }
+                int4 v[kMaxParts];   // under way together
+#pragma unroll
+                for (int p = 0; p < kMaxParts; ++p)
+                    if (p < parts) v[p] = *reinterpret_cast<const int4*>(cluster.map_shared_rank(partial, p) + t * kChannels + c4);
+#pragma unroll
+                for (int p = 0; p < kMaxParts; ++p)
+                    if (p < parts) { s[0] += v[p].x; s[1] += v[p].y; s[2] += v[p].z; s[3] += v[p].w; }
             } else {
                 for (int e = 0; e < 4; ++e)
-                    if (c0 + c4 + e < a.n) s[e] = dot_codes(a.x + (t0 + t) * a.x_stride, a.w + (c0 + c4 + e) * a.w_stride, a.k);
+                    if (c0 + c4 + e < a.n) s[e] = dot_codes(a.x + (long long)(t0 + t) * a.x_stride, a.w + (long long)(c0 + c4 + e) * a.w_stride, a.k);
             }
-            const float by = __ldg(a.x_scales + t0 + t);
             T* out = static_cast<T*>(a.out) + (long long)(t0 + t) * a.out_stride + c0 + c4;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c0 + c4 + e < a.n) out[e] = rounded<T>((float)s[e] * by * __ldg(a.w_scales + c0 + c4 + e));
+                if (c0 + c4 + e < a.n) out[e] = rounded<T>((float)s[e] * by * ws[e]);
         }
         cluster.sync();   // no block ends while another reads its sums
     } else if (gave_up) {
@@ -279,6 +293,261 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
             }
         }
     }
+}
+
+// ---- pairs of blocks ------------------------------------------------------------------------------------------------------------------------
+//
+// Many tokens: two blocks on neighbouring SMs take 256 channels and up to 256 tokens with one product (cta_group::2).  Each loads its 128 channels and half
+// of the tokens, a third less per product than a block alone, whose loads (96 bytes a clock at the tensor cores' rate) are more than an SM gets from L2.
+// The first block of the pair issues the products, when both blocks' loads have landed: they count on its barriers.
+constexpr int kPairMin = 192;              // tokens from which pairs are taken
+__device__ __forceinline__ uint32_t in_first(const void* p) {   // the address of the first block's copy of a shared variable
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_u32(p)));
+    return r;
+}
+__device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(tc::smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_umma(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {   // both blocks' barriers
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+
+// The tile's channels and tokens: 8 tiles of tokens beside one another share the channels that they read.
+__device__ __forceinline__ void place_of(const MatmulArgs& a, int tile, int* c0, int* t0) {
+    constexpr int kBeside = 8;
+    const int token_tiles = a.tiles / a.channel_tiles, band = kBeside * a.channel_tiles, first = tile / band * kBeside, beside = min(kBeside, token_tiles - first), i = tile % band;
+    *c0 = i / beside * (2 * kChannels);
+    *t0 = (first + i % beside) * a.tokens;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MatmulArgs a) {
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], ready[2], drained[2], last;
+    __shared__ uint32_t tmem_at;
+    __shared__ int gave_up;
+    __shared__ __align__(16) float s_scales[2][kMaxTokens];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster.block_rank();
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int mine = a.tokens / 2, stage_bytes = (kChannels + mine) * kSlab;   // of this block
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < a.stages; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&ready[i], 1); tc::mbar_init(&drained[i], 2 * kEpilogue); }
+        tc::mbar_init(&last, 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const int columns = tmem_columns(a.tokens, 2);
+    if (warp == kEpilogue + 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_at)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc::tc_fence_before();
+    cluster.sync();
+    tc::tc_fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp == kEpilogue) {
+        if (tc::elect_one()) {
+            int at = 0;
+            bool ok = true;
+            for (int tile = first; ok && tile < a.tiles; tile += step) {
+                int c0, t0;
+                place_of(a, tile, &c0, &t0);
+                for (int slab = 0; slab < a.slabs; ++slab, ++at) {
+                    const int st = at % a.stages;
+                    if (at >= a.stages && !tc::mbar_wait(&empty[st], (at / a.stages - 1) & 1, a.polls)) { ok = false; break; }
+                    if (rank == 0) tc::mbar_expect_tx(&full[st], 2 * stage_bytes);
+                    unsigned char* to = ring + st * stage_bytes;
+                    pair_load(to, &map_w, slab * kSlab, c0 + rank * kChannels, in_first(&full[st]));
+                    pair_load(to + kChannels * kSlab, &map_x, slab * kSlab, t0 + rank * mine, in_first(&full[st]));
+                }
+            }
+            if (!ok) {   // the loads under way land before the block ends (the second block's count here too, and are older than its wait that gave up)
+                gave_up = 1;
+                if (rank == 0)
+                    for (int i = max(0, at - a.stages); i < at; ++i) tc::mbar_wait(&full[i % a.stages], (i / a.stages) & 1, a.polls);
+            }
+        }
+        __syncwarp();
+    } else if (warp == kEpilogue + 1) {
+        if (rank == 0 && tc::elect_one()) {
+            const uint32_t idesc = idesc_i8(2 * kChannels, a.tokens);
+            int at = 0, count = 0;
+            bool ok = true;
+            for (int tile = first; ok && tile < a.tiles; tile += step, ++count) {
+                const int buf = count & 1;
+                if (count >= 2 && !tc::mbar_wait(&drained[buf], (count / 2 - 1) & 1, a.polls)) { ok = false; break; }
+                if (tile >= a.issued) { ok = false; break; }
+                tc::tc_fence_after();
+                for (int slab = 0; slab < a.slabs; ++slab, ++at) {
+                    const int st = at % a.stages;
+                    if (!tc::mbar_wait(&full[st], (at / a.stages) & 1, a.polls)) { ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t w_at = tc::smem_u32(ring + st * stage_bytes);
+                    const uint64_t dw = tc::make_sw128_desc(w_at), dx = tc::make_sw128_desc(w_at + kChannels * kSlab);
+#pragma unroll
+                    for (int q = 0; q < kSlab / 32; ++q) pair_umma(tmem + buf * a.tokens, dw + 2 * q, dx + 2 * q, idesc, slab > 0 || q > 0);
+                    pair_commit(&empty[st]);
+                }
+                if (ok) pair_commit(&ready[buf]);
+            }
+            if (!ok) {   // the products under way end before the tensor memory is freed
+                gave_up = 1;
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc::smem_u32(&last)) : "memory");
+                tc::mbar_wait(&last, 0, a.polls);
+            }
+        }
+        __syncwarp();
+    } else {
+        int count = 0;
+        for (int tile = first; tile < a.tiles; tile += step, ++count) {
+            const int buf = count & 1;
+            int c0, t0;
+            place_of(a, tile, &c0, &t0);
+            if (!tc::mbar_wait(&ready[buf], (count / 2) & 1, a.polls)) { gave_up = 1; break; }
+            __syncwarp();
+            tc::tc_fence_after();
+            const int quarter = warp & 3;
+            store_tile<T>(a, s_scales[count & 1], tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16), c0 + rank * kChannels + quarter * 32 + lane, t0, warp, lane);
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(&drained[buf])) : "memory");
+        }
+    }
+    tc::tc_fence_before();
+    cluster.sync();
+    tc::tc_fence_after();
+    if (warp == kEpilogue + 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    const int lost = gave_up | *cluster.map_shared_rank(&gave_up, rank ^ 1);
+    cluster.sync();   // neither block ends while the other looks
+    if (lost) {
+        for (int tile = first; tile < a.tiles; tile += step) {
+            int c0, t0;
+            place_of(a, tile, &c0, &t0);
+            for (int i = threadIdx.x; i < kChannels * a.tokens; i += kThreads) {
+                const int c = c0 + rank * kChannels + i % kChannels, t = t0 + i / kChannels;
+                if (c < a.n && t < a.m)
+                    static_cast<T*>(a.out)[(long long)t * a.out_stride + c] =
+                        rounded<T>((float)dot_codes(a.x + (long long)t * a.x_stride, a.w + (long long)c * a.w_stride, a.k) * __ldg(a.x_scales + t) * __ldg(a.w_scales + c));
+            }
+        }
+    }
+}
+
+// ---- few tokens -----------------------------------------------------------------------------------------------------------------------
+//
+// With up to 4 tokens the product is the reading of w, and the way to the tensor cores - a ring, tensor memory, an exchange between the blocks that
+// share a tile - is longer than the product itself.  Here a warp takes four channels and all tokens, 512 codes of each at a time, by dp4a; where channels
+// are few, several warps of a block share them along k and add their sums.
+constexpr int kFewTokens = 4;
+constexpr int kFewDepth = 1024;            // shorter rows leave lanes without work
+constexpr int kFewChannels = 4;            // a warp
+constexpr int kFewWarps = 8;               // a block
+
+__device__ __forceinline__ int dot16(int4 a, int4 b, int s) { return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, s)))); }
+
+// share: warps of a block that take the same channels.
+template <typename T, int M>
+__global__ void __launch_bounds__(32 * kFewWarps) k_i8_few_tokens(const MatmulArgs a, int share) {
+    __shared__ int s_sums[kFewWarps][kFewChannels * M];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share;
+    const long long c0 = ((long long)blockIdx.x * (kFewWarps / share) + warp / share) * kFewChannels;
+    int sums[kFewChannels][M] = {};
+    const signed char* w[kFewChannels];
+    const signed char* x[M];
+#pragma unroll
+    for (int c = 0; c < kFewChannels; ++c) w[c] = a.w + min(c0 + c, (long long)a.n - 1) * a.w_stride;   // (behind the last: the last, not written)
+#pragma unroll
+    for (int t = 0; t < M; ++t) x[t] = a.x + min(t, a.m - 1) * a.x_stride;
+    constexpr int kAhead = M <= 2 ? 4 : 2;      // rounds of loads at once
+    const int step = 512 * share;
+    int k0 = part * 512 + lane * 16;
+    const int whole = a.k - 15;                 // 16 codes from here on would pass the end
+    for (; k0 + (kAhead - 1) * step < whole; k0 += kAhead * step) {
+        int4 v[kAhead][kFewChannels];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int c = 0; c < kFewChannels; ++c) v[u][c] = __ldg(reinterpret_cast<const int4*>(w[c] + k0 + u * step));
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int t = 0; t < M; ++t) {
+                const int4 y = __ldg(reinterpret_cast<const int4*>(x[t] + k0 + u * step));
+#pragma unroll
+                for (int c = 0; c < kFewChannels; ++c) sums[c][t] = dot16(y, v[u][c], sums[c][t]);
+            }
+    }
+    for (; k0 < whole; k0 += step) {            // the last rounds
+        int4 v[kFewChannels];
+#pragma unroll
+        for (int c = 0; c < kFewChannels; ++c) v[c] = __ldg(reinterpret_cast<const int4*>(w[c] + k0));
+#pragma unroll
+        for (int t = 0; t < M; ++t) {
+            const int4 y = __ldg(reinterpret_cast<const int4*>(x[t] + k0));
+#pragma unroll
+            for (int c = 0; c < kFewChannels; ++c) sums[c][t] = dot16(y, v[c], sums[c][t]);
+        }
+    }
+    if (k0 < a.k) {                             // the last codes of the rows, fewer than 16
+#pragma unroll
+        for (int c = 0; c < kFewChannels; ++c)
+#pragma unroll
+            for (int t = 0; t < M; ++t) {
+                int s = sums[c][t];
+#pragma unroll 1
+                for (int i = k0; i < a.k; ++i) s += (int)w[c][i] * (int)x[t][i];
+                sums[c][t] = s;
+            }
+    }
+    // channel c, token t to lane c * M + t
+    int mine = 0;
+#pragma unroll
+    for (int c = 0; c < kFewChannels; ++c)
+#pragma unroll
+        for (int t = 0; t < M; ++t) {
+            const int s = __reduce_add_sync(0xffffffffu, sums[c][t]);
+            if (lane == c * M + t) mine = s;
+        }
+    const int c = lane / M, t = lane % M;
+    if (share > 1) {
+        if (lane < kFewChannels * M) s_sums[warp][lane] = mine;
+        __syncthreads();
+        if (part != 0 || lane >= kFewChannels * M) return;
+        for (int p = 1; p < share; ++p) mine += s_sums[warp + p][lane];
+    }
+    if (lane < kFewChannels * M && t < a.m && c0 + c < a.n)
+        static_cast<T*>(a.out)[(long long)t * a.out_stride + c0 + c] = rounded<T>((float)mine * __ldg(a.x_scales + t) * __ldg(a.w_scales + c0 + c));
+}
+
+template <typename T>
+psb_status run_few(const MatmulArgs& a, int sms, cudaStream_t s) {
+    const long long groups = ((long long)a.n + kFewChannels - 1) / kFewChannels;
+    int share = 1;
+    while (share < kFewWarps && groups * share < 16ll * sms && a.k > 512 * share) share *= 2;
+    const unsigned blocks = (unsigned)((groups * share + kFewWarps - 1) / kFewWarps);
+    switch (a.m) {
+        case 1: k_i8_few_tokens<T, 1><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
+        case 2: k_i8_few_tokens<T, 2><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
+        default: k_i8_few_tokens<T, 4><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
+    }
+    PSB_LAUNCH_CHECK();
+    count_launch();
+    return PSB_OK;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -314,19 +583,52 @@ psb_status codes_map(CUtensorMap* map, const void* base, int64_t rows, int k, in
 }
 
 template <typename T>
+psb_status run_pairs(MatmulArgs a, int sms, cudaStream_t s) {
+    const int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
+    a.tokens = ((a.m + token_tiles - 1) / token_tiles + 31) / 32 * 32;
+    a.channel_tiles = (a.n + 2 * kChannels - 1) / (2 * kChannels);
+    const long long tiles = (long long)token_tiles * a.channel_tiles;
+    if (tiles > 0x3fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^30 - 1 tiles of 256 x 256 outputs");
+    a.tiles = (int)tiles;
+    a.slabs = (a.k + kSlab - 1) / kSlab;
+    const int stage_bytes = (kChannels + a.tokens / 2) * kSlab;
+    a.stages = std::min(kMaxStages, kRing / stage_bytes);
+    const size_t smem = 1024 + (size_t)a.stages * stage_bytes;
+    CUtensorMap map_w, map_x;
+    PSB_TRY(codes_map(&map_w, a.w, a.n, a.k, a.w_stride, kChannels));
+    PSB_TRY(codes_map(&map_x, a.x, a.m, a.k, a.x_stride, a.tokens / 2));
+    PSB_TRY(kernel_shared(reinterpret_cast<const void*>(k_i8_matmul_pair<T>), smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.gridDim = dim3((unsigned)(2 * std::min<long long>(tiles, sms / 2)));
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    PSB_CUDA(cudaLaunchKernelEx(&cfg, k_i8_matmul_pair<T>, map_w, map_x, a));
+    count_launch();
+    return PSB_OK;
+}
+
+template <typename T>
 psb_status run(MatmulArgs a, int sms, cudaStream_t s) {
+    // (k = 4,096, by dp4a and on the tensor cores: 1 token and 32,000 channels 21.7 and 25.7 us, 4,096 channels 5.9 and 7.1; 4 tokens and 32,000
+    // channels 30.4 and 26.5, 4,096 channels 5.4 and 7.4)
+    const bool few = a.m <= 2 || (a.m <= kFewTokens && a.n <= kChannels * (sms / 2));
+    if (few && a.k >= kFewDepth && a.issued == kAllTiles) return run_few<T>(a, sms, s);
     // tiles of tokens of even size, each a multiple of 16
     const int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
     a.tokens = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
     a.channel_tiles = (a.n + kChannels - 1) / kChannels;
     const long long tiles = (long long)token_tiles * a.channel_tiles;
+    if (a.m >= kPairMin && tiles >= 2 * sms) return run_pairs<T>(a, sms, s);
     if (tiles > 0x7fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^31 - 1 tiles of 128 x 256 outputs");
     a.tiles = (int)tiles;
     a.slabs = (a.k + kSlab - 1) / kSlab;
     int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= sms && a.slabs >= parts * 4) parts *= 2;
+    while (parts < kMaxParts && tiles * parts * 2 <= sms && a.slabs >= parts * 4) parts *= 2;
     const int stage_bytes = (kChannels + a.tokens) * kSlab;
-    a.stages = std::min(kMaxStages, kRing / stage_bytes);
+    a.stages = std::min(std::min(kMaxStages, std::max(2, (a.slabs + parts - 1) / parts)), kRing / stage_bytes);
     const size_t smem = 1024 + std::max((size_t)a.stages * stage_bytes, parts > 1 ? (size_t)a.tokens * kChannels * 4 : 0);
     CUtensorMap map_w, map_x;
     PSB_TRY(codes_map(&map_w, a.w, a.n, a.k, a.w_stride, kChannels));
@@ -396,13 +698,13 @@ extern "C" {
 
 psb_status psb_i8_matmul(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride, const float* d_w_scales, int64_t n,
                          int k, void* d_out, int out_type, int64_t out_stride, int device, void* stream) {
-    return matmul(d_x, x_stride, d_x_scales, m, d_w, w_stride, d_w_scales, n, k, d_out, out_type, out_stride, 0x7fffffffffffffffll, kWaitPolls, device, stream);
+    return matmul(d_x, x_stride, d_x_scales, m, d_w, w_stride, d_w_scales, n, k, d_out, out_type, out_stride, kAllTiles, kWaitPolls, device, stream);
 }
 
 psb_status psb_i8_matmul_limited(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride, const float* d_w_scales,
                                  int64_t n, int k, void* d_out, int out_type, int64_t out_stride, int64_t tiles, int polls, int device, void* stream) {
     if (polls <= 0) return fail(PSB_INVALID_ARGUMENT, "product of codes: a wait without polls");
-    return matmul(d_x, x_stride, d_x_scales, m, d_w, w_stride, d_w_scales, n, k, d_out, out_type, out_stride, tiles < 0 ? 0x7fffffffffffffffll : tiles, polls, device,
+    return matmul(d_x, x_stride, d_x_scales, m, d_w, w_stride, d_w_scales, n, k, d_out, out_type, out_stride, tiles < 0 ? kAllTiles : tiles, polls, device,
                   stream);
 }
 

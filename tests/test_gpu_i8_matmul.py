@@ -47,14 +47,16 @@ def check(psb, m, n, k, t, x_pad=0, w_pad=0, out_pad=0, full=False, limited=None
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 128), (1, 1000, 4096), (2, 129, 16), (16, 128, 100), (17, 127, 129), (31, 300, 31), (64, 64, 2048), (100, 513, 640),
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 128), (1, 1000, 4096), (1, 3, 5000), (2, 1001, 1037), (3, 515, 2063), (4, 30, 8200), (4, 10000, 1024), (2, 129, 16), (16, 128, 100), (17, 127, 129), (31, 300, 31), (64, 64, 2048), (100, 513, 640),
                                    (128, 128, 128), (129, 257, 257), (255, 100, 33), (256, 256, 512), (257, 130, 1000), (300, 5000, 96), (513, 640, 300),
                                    (1000, 2000, 130), (3, 40000, 256), (70, 130, 20000), (2049, 70, 72)])
 def test_products(psb, m, n, k, t):
     check(psb, m, n, k, t)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (37, 4099, 4000), (256, 2048, 8192), (4096, 4096, 1024), (2500, 3001, 515), (600, 30000, 128)])
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (37, 4099, 4000), (256, 2048, 8192), (4096, 4096, 1024), (2500, 3001, 515), (600, 30000, 128),
+                                   # pairs of blocks: odd sizes, one slab, last tiles of few channels and tokens
+                                   (193, 40000, 100), (4097, 5001, 333), (5000, 2561, 129), (300, 20000, 2048), (10000, 1100, 16)])
 def test_larger_products(psb, m, n, k):
     check(psb, m, n, k, torch.float32)
     check(psb, m, n, k, torch.bfloat16)
@@ -80,7 +82,8 @@ def test_codes_behind_a_row_do_not_count(psb):
 
 
 @pytest.mark.parametrize("m,n,k,tiles", [(1, 300, 512, 0), (1, 300, 512, 1), (40, 130, 4096, 0), (300, 500, 700, 3), (300, 500, 700, 0), (2000, 4000, 128, 200),
-                                         (2000, 4000, 1100, 150), (520, 70, 5000, 0)])
+                                         (2000, 4000, 1100, 150), (520, 70, 5000, 0),
+                                         (3000, 4000, 300, 0), (3000, 4000, 300, 130), (700, 20000, 1000, 80)])
 def test_results_when_a_wait_gives_up(psb, m, n, k, tiles):
     for t in TYPES:
         check(psb, m, n, k, t, limited=tiles)
