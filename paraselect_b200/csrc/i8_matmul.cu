@@ -95,18 +95,28 @@ __device__ int dot_codes(const signed char* a, const signed char* b, int k) {
     return s;
 }
 
-// An epilogue warp's half of the columns of a tile, 32 channels: channel c in this thread, tokens from t0.  Every epilogue warp of the block calls it.
+// The scales that a thread of the epilogue needs for a tile: its channel's and one token's.  They are read a tile ahead: a tile of one slab took 0.95 us, most of
+// which was the way of its scales from memory (8 x 500,000 x 128: 27 us).
+struct Scales { float w, x; };
+__device__ __forceinline__ Scales scales_of(const MatmulArgs& a, bool there, int c, int t0, int token) {
+    return Scales{there && c < a.n ? __ldg(a.w_scales + c) : 0.f, there && token < a.tokens && t0 + token < a.m ? __ldg(a.x_scales + t0 + token) : 0.f};
+}
+
+// An epilogue warp's columns of a tile, 32 channels: channel c in this thread, tokens from t0.  SOLO: the four warps of this half of the epilogue have the tile
+// to themselves (its tokens are 32 at most), otherwise each half takes every other 16 tokens; all warps that share the tile call it.
 // `scales`: the other of the two buffers still serves slower warps' last tile.
-template <typename T>
-__device__ __forceinline__ void store_tile(const MatmulArgs& a, float* scales, uint32_t from, int c, int t0, int warp, int lane) {
-    const int half = warp >> 2, i0 = warp * 32 + lane;
-    if (i0 < a.tokens) scales[i0] = t0 + i0 < a.m ? __ldg(a.x_scales + t0 + i0) : 0.f;
+template <typename T, bool SOLO>
+__device__ __forceinline__ void store_tile(const MatmulArgs& a, float* scales, const Scales& own, uint32_t from, int c, int t0, int warp, int lane) {
+    const int half = SOLO ? 0 : warp >> 2, every = SOLO ? 16 : 32;
+    if (SOLO) scales += warp >> 2 << 7;
+    scales[(SOLO ? warp & 3 : warp) * 32 + lane] = own.x;
     const bool here = c < a.n;
-    const float ws = here ? __ldg(a.w_scales + c) : 0.f;
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogue) : "memory");
+    const float ws = own.w;
+    if (SOLO) asm volatile("bar.sync %0, %1;" ::"r"(1 + (warp >> 2)), "n"(16 * kEpilogue) : "memory");
+    else asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogue) : "memory");
     T* out = static_cast<T*>(a.out) + (long long)(t0 + half * 16) * a.out_stride + c;
     const int live = min(a.tokens, a.m - t0);
-    for (int t = half * 16; t < live; t += 32, out += 32 * a.out_stride) {
+    for (int t = half * 16; t < live; t += every, out += every * a.out_stride) {
         uint32_t v[16];
         tmem_ld16(from + t, v);
         float by[16];
@@ -145,9 +155,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     const int slab0 = a.slabs * part / parts, slab1 = a.slabs * (part + 1) / parts;
     const int stage_bytes = (kChannels + a.tokens) * kSlab;
     constexpr int kBuffers = SPLIT ? 1 : 2;
+    // Tiles of few tokens go to the two halves of the epilogue in turn: what a tile takes is then the way from barrier to barrier, not its stores
+    // (8 x 500,000 x 128: 24.6 us with both at each tile).
+    const bool solo = !SPLIT && a.tokens <= 32;
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) { tc::mbar_init(&full[i], 1); tc::mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(&ready[i], 1); tc::mbar_init(&drained[i], kEpilogue); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&ready[i], 1); tc::mbar_init(&drained[i], solo ? kEpilogue / 2 : kEpilogue); }
         tc::mbar_init(&last, 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -217,9 +230,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
         __syncwarp();
     } else {
         int count = 0;
-        for (int tile = first; tile < a.tiles; tile += step, ++count) {
+        const int turns = solo ? 2 : 1;
+        auto scales = [&](int tile) {
+            return scales_of(a, !SPLIT && tile < a.tiles, tile % a.channel_tiles * kChannels + (warp & 3) * 32 + lane, tile / a.channel_tiles * a.tokens, (solo ? warp & 3 : warp) * 32 + lane);
+        };
+        if (solo) count = warp >> 2;
+        int tile = first + count * step;
+        Scales next = scales(tile);
+        for (; tile < a.tiles; tile += turns * step, count += turns) {
             const int buf = count % kBuffers;
             const int c0 = tile % a.channel_tiles * kChannels, t0 = tile / a.channel_tiles * a.tokens;
+            const Scales own = next;
+            next = scales(tile + turns * step);
             if (!tc::mbar_wait(&ready[buf], (count / kBuffers) & 1, a.polls)) { gave_up = 1; break; }
             __syncwarp();
             tc::tc_fence_after();
@@ -236,7 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
                     for (int i = 0; i < 16; ++i) partial[(t + i) * kChannels + c] = (int)v[i];
                 }
             } else {
-                store_tile<T>(a, s_scales[count & 1], from, c0 + c, t0, warp, lane);
+                if (solo) store_tile<T, true>(a, s_scales[count / 2 & 1], own, from, c0 + c, t0, warp, lane);
+                else store_tile<T, false>(a, s_scales[count & 1], own, from, c0 + c, t0, warp, lane);
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&drained[buf])) : "memory");
@@ -414,15 +437,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
         __syncwarp();
     } else {
         int count = 0;
+        auto scales = [&](int tile) {
+            int c0 = 0, t0 = 0;
+            if (tile < a.tiles) place_of(a, tile, &c0, &t0);
+            return scales_of(a, tile < a.tiles, c0 + rank * kChannels + (warp & 3) * 32 + lane, t0, warp * 32 + lane);
+        };
+        Scales next = scales(first);
         for (int tile = first; tile < a.tiles; tile += step, ++count) {
             const int buf = count & 1;
             int c0, t0;
             place_of(a, tile, &c0, &t0);
+            const Scales own = next;
+            next = scales(tile + step);
             if (!tc::mbar_wait(&ready[buf], (count / 2) & 1, a.polls)) { gave_up = 1; break; }
             __syncwarp();
             tc::tc_fence_after();
             const int quarter = warp & 3;
-            store_tile<T>(a, s_scales[count & 1], tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16), c0 + rank * kChannels + quarter * 32 + lane, t0, warp, lane);
+            store_tile<T, false>(a, s_scales[count & 1], own, tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16), c0 + rank * kChannels + quarter * 32 + lane, t0, warp, lane);
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(&drained[buf])) : "memory");
@@ -450,22 +481,48 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
 
 // ---- few tokens -----------------------------------------------------------------------------------------------------------------------
 //
-// With up to 4 tokens the product is the reading of w, and the way to the tensor cores - a ring, tensor memory, an exchange between the blocks that
+// With few tokens the product is the reading of w, and the way to the tensor cores - a ring, tensor memory, an exchange between the blocks that
 // share a tile - is longer than the product itself.  Here a warp takes four channels and all tokens, 512 codes of each at a time, by dp4a; where channels
 // are few, several warps of a block share them along k and add their sums.
 constexpr int kFewTokens = 4;
-constexpr int kFewDepth = 1024;            // shorter rows leave lanes without work
+constexpr int kFewDepth = 128;
 constexpr int kFewChannels = 4;            // a warp
 constexpr int kFewWarps = 8;               // a block
 
 __device__ __forceinline__ int dot16(int4 a, int4 b, int s) { return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, s)))); }
 
-// share: warps of a block that take the same channels.
-template <typename T, int M>
+// w's codes pass through L1 once: x's stay there.  (With more tokens the compiler then waits for each load before the next: plain ones.)
+template <int M>
+__device__ __forceinline__ int4 stream16(const signed char* at) {
+    if constexpr (M > 1) return __ldg(reinterpret_cast<const int4*>(at));
+    int4 v;
+    asm("ld.global.nc.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+    return v;
+}
+
+// The codes of a row of k from `at` on, fewer than 16, and whatever lies behind them: what belongs to the row's stride can be read, but behind the last row
+// there may be nothing.
+__device__ __forceinline__ int4 last16(const signed char* row, int at, int k, bool inner) {
+    if (inner) return __ldg(reinterpret_cast<const int4*>(row + at));
+    unsigned v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 15; ++i)
+        if (at + i < k) v[i >> 2] |= (unsigned)(unsigned char)row[at + i] << 8 * (i & 3);
+    return make_int4((int)v[0], (int)v[1], (int)v[2], (int)v[3]);
+}
+// The first n codes, zeros behind them.
+__device__ __forceinline__ int4 codes_of(int4 v, int n) {
+    auto word = [&](int w, int from) { const int bytes = n - from; return bytes >= 4 ? w : bytes <= 0 ? 0 : w & (int)((1u << 8 * bytes) - 1); };
+    return make_int4(word(v.x, 0), word(v.y, 4), word(v.z, 8), word(v.w, 12));
+}
+
+// LANES of a warp take four channels, 16 codes a lane at a time.  share: warps of a block that take the same channels.
+template <typename T, int M, int LANES>
 __global__ void __launch_bounds__(32 * kFewWarps) k_i8_few_tokens(const MatmulArgs a, int share) {
-    __shared__ int s_sums[kFewWarps][kFewChannels * M];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share;
-    const long long c0 = ((long long)blockIdx.x * (kFewWarps / share) + warp / share) * kFewChannels;
+    constexpr int kGroups = 32 / LANES;
+    __shared__ int s_sums[kFewWarps][kGroups * kFewChannels * M];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share, group = lane / LANES, in = lane % LANES;
+    const long long c0 = (((long long)blockIdx.x * (kFewWarps / share) + warp / share) * kGroups + group) * kFewChannels;
     int sums[kFewChannels][M] = {};
     const signed char* w[kFewChannels];
     const signed char* x[M];
@@ -474,15 +531,15 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_i8_few_tokens(const MatmulAr
 #pragma unroll
     for (int t = 0; t < M; ++t) x[t] = a.x + min(t, a.m - 1) * a.x_stride;
     constexpr int kAhead = M <= 2 ? 4 : 2;      // rounds of loads at once
-    const int step = 512 * share;
-    int k0 = part * 512 + lane * 16;
+    const int step = LANES * 16 * share;
+    int k0 = (part * LANES + in) * 16;
     const int whole = a.k - 15;                 // 16 codes from here on would pass the end
     for (; k0 + (kAhead - 1) * step < whole; k0 += kAhead * step) {
         int4 v[kAhead][kFewChannels];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-            for (int c = 0; c < kFewChannels; ++c) v[u][c] = __ldg(reinterpret_cast<const int4*>(w[c] + k0 + u * step));
+            for (int c = 0; c < kFewChannels; ++c) v[u][c] = stream16<M>(w[c] + k0 + u * step);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
 #pragma unroll
@@ -495,7 +552,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_i8_few_tokens(const MatmulAr
     for (; k0 < whole; k0 += step) {            // the last rounds
         int4 v[kFewChannels];
 #pragma unroll
-        for (int c = 0; c < kFewChannels; ++c) v[c] = __ldg(reinterpret_cast<const int4*>(w[c] + k0));
+        for (int c = 0; c < kFewChannels; ++c) v[c] = stream16<M>(w[c] + k0);
 #pragma unroll
         for (int t = 0; t < M; ++t) {
             const int4 y = __ldg(reinterpret_cast<const int4*>(x[t] + k0));
@@ -504,50 +561,70 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_i8_few_tokens(const MatmulAr
         }
     }
     if (k0 < a.k) {                             // the last codes of the rows, fewer than 16
+        int4 v[kFewChannels];
 #pragma unroll
-        for (int c = 0; c < kFewChannels; ++c)
+        for (int c = 0; c < kFewChannels; ++c) v[c] = last16(w[c], k0, a.k, c0 + c < a.n - 1);
 #pragma unroll
-            for (int t = 0; t < M; ++t) {
-                int s = sums[c][t];
-#pragma unroll 1
-                for (int i = k0; i < a.k; ++i) s += (int)w[c][i] * (int)x[t][i];
-                sums[c][t] = s;
-            }
+        for (int t = 0; t < M; ++t) {
+            const int4 y = codes_of(last16(x[t], k0, a.k, t < a.m - 1), a.k - k0);
+#pragma unroll
+            for (int c = 0; c < kFewChannels; ++c) sums[c][t] = dot16(y, v[c], sums[c][t]);
+        }
     }
-    // channel c, token t to lane c * M + t
-    int mine = 0;
+    // channel c and token t of a group to its lane (c * M + t) % LANES, in turn (c * M + t) / LANES
+    constexpr int kTurns = (kFewChannels * M + LANES - 1) / LANES;
+    int mine[kTurns] = {};
+    __syncwarp();
 #pragma unroll
     for (int c = 0; c < kFewChannels; ++c)
 #pragma unroll
         for (int t = 0; t < M; ++t) {
-            const int s = __reduce_add_sync(0xffffffffu, sums[c][t]);
-            if (lane == c * M + t) mine = s;
+            int s = sums[c][t];
+            if constexpr (LANES == 32) s = __reduce_add_sync(0xffffffffu, s);
+            else
+#pragma unroll
+                for (int o = LANES >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            const int i = c * M + t;
+            if (in == i % LANES) mine[i / LANES] = s;
         }
-    const int c = lane / M, t = lane % M;
     if (share > 1) {
-        if (lane < kFewChannels * M) s_sums[warp][lane] = mine;
+#pragma unroll
+        for (int j = 0; j < kTurns; ++j)
+            if (in + j * LANES < kFewChannels * M) s_sums[warp][group * kFewChannels * M + in + j * LANES] = mine[j];
         __syncthreads();
-        if (part != 0 || lane >= kFewChannels * M) return;
-        for (int p = 1; p < share; ++p) mine += s_sums[warp + p][lane];
+        if (part != 0) return;
     }
-    if (lane < kFewChannels * M && t < a.m && c0 + c < a.n)
-        static_cast<T*>(a.out)[(long long)t * a.out_stride + c0 + c] = rounded<T>((float)mine * __ldg(a.x_scales + t) * __ldg(a.w_scales + c0 + c));
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j) {
+        const int i = in + j * LANES, c = i / M, t = i % M;
+        if (i >= kFewChannels * M || t >= a.m || c0 + c >= a.n) continue;
+        for (int p = 1; p < share; ++p) mine[j] += s_sums[warp + p][group * kFewChannels * M + i];
+        static_cast<T*>(a.out)[(long long)t * a.out_stride + c0 + c] = rounded<T>((float)mine[j] * __ldg(a.x_scales + t) * __ldg(a.w_scales + c0 + c));
+    }
 }
 
-template <typename T>
-psb_status run_few(const MatmulArgs& a, int sms, cudaStream_t s) {
-    const long long groups = ((long long)a.n + kFewChannels - 1) / kFewChannels;
+template <typename T, int M>
+psb_status start_few(const MatmulArgs& a, int sms, cudaStream_t s) {
+    int lanes = 4;   // as many as have codes
+    while (lanes < 32 && a.k > lanes * 24) lanes *= 2;
+    const long long groups = ((long long)a.n + kFewChannels * (32 / lanes) - 1) / (kFewChannels * (32 / lanes));   // warps
     int share = 1;
-    while (share < kFewWarps && groups * share < 16ll * sms && a.k > 512 * share) share *= 2;
+    while (share < kFewWarps && groups * share < 16ll * sms && a.k > lanes * 16 * share) share *= 2;
     const unsigned blocks = (unsigned)((groups * share + kFewWarps - 1) / kFewWarps);
-    switch (a.m) {
-        case 1: k_i8_few_tokens<T, 1><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
-        case 2: k_i8_few_tokens<T, 2><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
-        default: k_i8_few_tokens<T, 4><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
+    switch (lanes) {
+        case 4: k_i8_few_tokens<T, M, 4><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
+        case 8: k_i8_few_tokens<T, M, 8><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
+        case 16: k_i8_few_tokens<T, M, 16><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
+        default: k_i8_few_tokens<T, M, 32><<<blocks, 32 * kFewWarps, 0, s>>>(a, share); break;
     }
     PSB_LAUNCH_CHECK();
     count_launch();
     return PSB_OK;
+}
+
+template <typename T>
+psb_status run_few(const MatmulArgs& a, int sms, cudaStream_t s) {
+    return a.m == 1 ? start_few<T, 1>(a, sms, s) : a.m == 2 ? start_few<T, 2>(a, sms, s) : start_few<T, 4>(a, sms, s);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -614,14 +691,15 @@ template <typename T>
 psb_status run(MatmulArgs a, int sms, cudaStream_t s) {
     // (k = 4,096, by dp4a and on the tensor cores: 1 token and 32,000 channels 21.7 and 25.7 us, 4,096 channels 5.9 and 7.1; 4 tokens and 32,000
     // channels 30.4 and 26.5, 4,096 channels 5.4 and 7.4)
-    const bool few = a.m <= 2 || (a.m <= kFewTokens && a.n <= kChannels * (sms / 2));
-    if (few && a.k >= kFewDepth && a.issued == kAllTiles) return run_few<T>(a, sms, s);
-    // tiles of tokens of even size, each a multiple of 16
-    const int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
-    a.tokens = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    const bool few = a.m == 1 || (a.m <= kFewTokens && (a.n <= kChannels * (sms / 2) || a.k <= kFewDepth));
+    if (few && a.issued == kAllTiles) return run_few<T>(a, sms, s);
+    // tiles of tokens of even size, each a multiple of 16: of 256 at most, or of 128 where they would not fill half of the GPU
     a.channel_tiles = (a.n + kChannels - 1) / kChannels;
+    int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
+    if (token_tiles > 1 && (long long)token_tiles * a.channel_tiles * 2 < sms) token_tiles = (a.m + 127) / 128;
+    a.tokens = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
     const long long tiles = (long long)token_tiles * a.channel_tiles;
-    if (a.m >= kPairMin && tiles >= 2 * sms) return run_pairs<T>(a, sms, s);
+    if (a.m >= kPairMin && tiles * 2 >= sms) return run_pairs<T>(a, sms, s);
     if (tiles > 0x7fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^31 - 1 tiles of 128 x 256 outputs");
     a.tiles = (int)tiles;
     a.slabs = (a.k + kSlab - 1) / kSlab;
