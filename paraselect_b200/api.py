@@ -867,48 +867,52 @@ def _call(name, *args):
         f.argtypes = _OPERATOR_ARGS[name]
         fn = _operators[name] = (_lib, f)
     status = fn[1](*args)
-    if status != PSB_OK:
+    if status:
         _check(status)
+
+
+def _at(tensor):
+    """Address of a device tensor, or None."""
+    return None if tensor is None else tensor.data_ptr()
 
 
 def i8_encode_rows(d_rows, n, dim, d_codes, d_scales, row_stride=0, code_stride=0, device=0, stream=None):
     """8-bit codes of n rows and a scale for each: row = codes * scale.  Strides in elements (0 = the rows lie side by side)."""
-    _call("psb_i8_encode_rows", _p(d_rows), _type(d_rows), n, dim, row_stride or dim, _p(d_codes), code_stride or dim, _p(d_scales), device, stream)
+    _call("psb_i8_encode_rows", _at(d_rows), _type(d_rows), n, dim, row_stride or dim, _at(d_codes), code_stride or dim, _at(d_scales), device, stream)
 
 
 def i8_norm_rows(d_rows, n, dim, d_weight, eps, d_codes, d_scales, d_residual=None, d_sum=None, row_stride=0, residual_stride=0,
                  sum_stride=0, code_stride=0, device=0, stream=None):
     """8-bit codes of the root-mean-square norm of rows + residual; d_sum receives the sum, and may be d_rows or d_residual."""
-    kind = _type(d_rows)
-    for t in (d_weight, d_residual, d_sum):
-        if t is not None and _type(t) != kind:
-            raise InvalidArgument(1, "rows, weight, residual and sum are of one type")
-    _call("psb_i8_norm_rows", _p(d_rows), _p(d_residual), _p(d_weight), kind, n, dim, row_stride or dim, residual_stride or dim, eps,
-          _p(d_sum), sum_stride or dim, _p(d_codes), code_stride or dim, _p(d_scales), device, stream)
+    kind, dtype = _type(d_rows), d_rows.dtype
+    if (d_weight is not None and d_weight.dtype != dtype) or (d_residual is not None and d_residual.dtype != dtype) or (d_sum is not None and d_sum.dtype != dtype):
+        raise InvalidArgument(1, "rows, weight, residual and sum are of one type")
+    _call("psb_i8_norm_rows", _at(d_rows), _at(d_residual), _at(d_weight), kind, n, dim, row_stride or dim, residual_stride or dim, eps,
+          _at(d_sum), sum_stride or dim, _at(d_codes), code_stride or dim, _at(d_scales), device, stream)
 
 
 def i8_matmul(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, x_stride=0, w_stride=0, out_stride=0, device=0, stream=None):
     """out [m][n] = the products of m and n rows of k codes, with both sides' scales."""
-    _call("psb_i8_matmul", _p(d_x), x_stride or k, _p(d_x_scales), m, _p(d_w), w_stride or k, _p(d_w_scales), n, k, _p(d_out), _type(d_out),
+    _call("psb_i8_matmul", _at(d_x), x_stride or k, _at(d_x_scales), m, _at(d_w), w_stride or k, _at(d_w_scales), n, k, _at(d_out), _type(d_out),
           out_stride or n, device, stream)
 
 
 def i8_matmul_limited(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, tiles=-1, polls=1 << 22, x_stride=0, w_stride=0, out_stride=0,
                       device=0, stream=None):
     """Test hook of i8_matmul's time-out path; see include/psb.h."""
-    _call("psb_i8_matmul_limited", _p(d_x), x_stride or k, _p(d_x_scales), m, _p(d_w), w_stride or k, _p(d_w_scales), n, k, _p(d_out),
+    _call("psb_i8_matmul_limited", _at(d_x), x_stride or k, _at(d_x_scales), m, _at(d_w), w_stride or k, _at(d_w_scales), n, k, _at(d_out),
           _type(d_out), out_stride or n, tiles, polls, device, stream)
 
 
 def beam_select(d_logits, d_scores, batch, beams, vocab, k, d_parents, d_tokens, d_totals, row_stride=0, device=0, stream=None):
     """The k best continuations of every item over its beams and the vocabulary: parents and tokens [batch][k] int32, totals fp32."""
-    _call("psb_beam_select", _p(d_logits), _type(d_logits), row_stride or vocab, _p(d_scores), batch, beams, vocab, k, _p(d_parents),
-          _p(d_tokens), _p(d_totals), device, stream)
+    _call("psb_beam_select", _at(d_logits), _type(d_logits), row_stride or vocab, _at(d_scores), batch, beams, vocab, k, _at(d_parents),
+          _at(d_tokens), _at(d_totals), device, stream)
 
 
 def beam_reorder(d_in, d_out, d_parents, layers, batch, beams, heads, tokens, token_bytes, d_lengths=None, device=0, stream=None):
     """States [layers][batch][beams][heads][tokens][token_bytes] in the order of the chosen parents; d_out may be d_in."""
-    _call("psb_beam_reorder", _p(d_in), _p(d_out), _p(d_parents), layers, batch, beams, heads, tokens, token_bytes, _p(d_lengths), device, stream)
+    _call("psb_beam_reorder", _at(d_in), _at(d_out), _at(d_parents), layers, batch, beams, heads, tokens, token_bytes, _at(d_lengths), device, stream)
 
 
 def gen_mixture_rows(d_centres, d_offsets, ncomp, dim, sigma, seed, row_begin, n, d_out, device=0, stream=None):

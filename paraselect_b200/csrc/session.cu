@@ -179,7 +179,10 @@ psb_status check_device(int device, int* sm_count = nullptr) {
 psb_status DeviceScope::enter(int device) {
     int now = -1;
     if (cudaGetDevice(&now) != cudaSuccess) { cudaGetLastError(); now = -1; }   // check_device says what is wrong
+    static std::atomic<int> seen[64];   // multiprocessors of the devices that check_device has let through: it costs a call of microseconds a tenth
+    if (now == device && device >= 0 && device < 64 && (sms = seen[device].load(std::memory_order_relaxed)) > 0) return PSB_OK;
     PSB_TRY(check_device(device, &sms));
+    if (device < 64) seen[device].store(sms, std::memory_order_relaxed);
     if (now != device) before = now;
     return PSB_OK;
 }
