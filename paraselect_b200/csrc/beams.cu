@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -477,7 +478,16 @@ psb_status select(SelectArgs a, int batch, int sms, cudaStream_t s) {
     while (a.groups > 1 && a.per_beam * a.beams * a.groups > kMaxGroups) a.groups /= 2;
     const void* kernel = reinterpret_cast<const void*>(k_beam_select<T>);
     PSB_TRY(kernel_shared(kernel, sizeof(SelectShared)));
-    if (blocks > 8) PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (blocks > 8) {   // clusters of more than 8 are asked for once a device
+        static std::atomic<unsigned long long> asked{0};
+        int device = 0;
+        PSB_CUDA(cudaGetDevice(&device));
+        const unsigned long long bit = device < 64 ? 1ull << device : 0;
+        if (!(asked.load(std::memory_order_relaxed) & bit)) {
+            PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            asked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(batch * blocks)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = sizeof(SelectShared); cfg.stream = s;
     cudaLaunchAttribute attr = {};

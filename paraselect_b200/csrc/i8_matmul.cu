@@ -700,7 +700,7 @@ psb_status run(MatmulArgs a, int sms, cudaStream_t s) {
     a.tokens = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
     const long long tiles = (long long)token_tiles * a.channel_tiles;
     if (a.m >= kPairMin && tiles * 2 >= sms) return run_pairs<T>(a, sms, s);
-    if (tiles > 0x7fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^31 - 1 tiles of 128 x 256 outputs");
+    if (tiles > 0x3fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^30 - 1 tiles of 128 x 256 outputs");
     a.tiles = (int)tiles;
     a.slabs = (a.k + kSlab - 1) / kSlab;
     int parts = 1;
