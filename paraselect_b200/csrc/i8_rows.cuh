@@ -46,17 +46,14 @@ template <typename T> struct Pack {
     __device__ __forceinline__ void read_again(const T* row, int at) {
         asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(word[0]), "=r"(word[1]), "=r"(word[2]), "=r"(word[3]) : "l"(row + at));
     }
-    // Those of them that a row of dim elements has, wherever it begins; the others are left as they are.
-    __device__ __forceinline__ void read_each(const T* row, int at, int dim) {
+    __device__ __forceinline__ void read_each(const T* row, int at) {   // wherever the row begins
+        T v[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-            if (at + e >= 0 && at + e < dim) put(e, row[at + e]);
-    }
-    __device__ __forceinline__ void put(int e, T v) {
-        if constexpr (sizeof(T) == 4) word[e] = *reinterpret_cast<const unsigned*>(&v);
-        else {
-            const unsigned u = *reinterpret_cast<const unsigned short*>(&v);
-            word[e >> 1] = e & 1 ? (word[e >> 1] & 0xffffu) | u << 16 : (word[e >> 1] & 0xffff0000u) | u;
+        for (int e = 0; e < VEC; ++e) v[e] = row[at + e];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) word[i] = *reinterpret_cast<const unsigned*>(&v[i]);
+            else word[i] = *reinterpret_cast<const unsigned short*>(&v[2 * i]) | (unsigned)*reinterpret_cast<const unsigned short*>(&v[2 * i + 1]) << 16;
         }
     }
     __device__ __forceinline__ void zeros() { set(make_uint4(0, 0, 0, 0)); }
@@ -70,22 +67,16 @@ template <typename T> struct Pack {
         else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e & 1 ? word[e >> 1] & 0xffff0000u : word[e >> 1] << 16);
         else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&word[e >> 1])); return e & 1 ? f.y : f.x; }
     }
-    template <bool SHIFT> static __device__ __forceinline__ void write(T* row, int at, int dim, const unsigned long long* pairs) {
-        if (!SHIFT || (at >= 0 && at + VEC <= dim)) {
-            unsigned o[4];
+    static __device__ __forceinline__ void write(T* at, const unsigned long long* pairs) {
+        unsigned o[4];
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-                const float2 v = halves(pairs[i]);
-                if constexpr (sizeof(T) == 4) { o[2 * i] = __float_as_uint(v.x); o[2 * i + 1] = __float_as_uint(v.y); }
-                else if constexpr (std::is_same<T, __nv_bfloat16>::value) { const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y); o[i] = *reinterpret_cast<const unsigned*>(&p); }
-                else { const __half2 p = __floats2half2_rn(v.x, v.y); o[i] = *reinterpret_cast<const unsigned*>(&p); }
-            }
-            *reinterpret_cast<uint4*>(row + at) = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (at + e >= 0 && at + e < dim) { const float2 v = halves(pairs[e / 2]); row[at + e] = from_float<T>(e & 1 ? v.y : v.x); }
+        for (int i = 0; i < VEC / 2; ++i) {
+            const float2 v = halves(pairs[i]);
+            if constexpr (sizeof(T) == 4) { o[2 * i] = __float_as_uint(v.x); o[2 * i + 1] = __float_as_uint(v.y); }
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) { const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y); o[i] = *reinterpret_cast<const unsigned*>(&p); }
+            else { const __half2 p = __floats2half2_rn(v.x, v.y); o[i] = *reinterpret_cast<const unsigned*>(&p); }
         }
+        *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 };
 
@@ -142,11 +133,11 @@ template <int kEach, int MOST, bool NORM> constexpr int blocks_of() { return MOS
 // it.  Code for it beside every element took five times the kernel's time, and a thread of its own for it half of the rest, the block waiting
 // (16,384 rows of 8,192 in bf16: 789 and 499 us).  fp32 arithmetic goes two elements an instruction: the kernel was bound by issue (239 us).
 //
-// SHIFT: rows that begin anywhere.  Packs are those of memory, so that the row begins in the middle of its first and ends in the middle of its last, at
-// the same places in all rows of a block.  Those two are read and written element by element.  With a weight, whose packs lie otherwise, a block takes
-// every G-th row, G a multiple of a pack's elements, so that the weight is laid out once, in shared memory; the two packs are then read whole, but for
-// the first row's first and the last row's last, and what belongs to the neighbouring rows is put to zero.  (7,000 rows of 8,191 in bf16 element by
-// element: 317 us, with the weight's packs shifted anew for each row 273, so 127.  Rows that begin at packs lose by keeping the weight: 74 us and 82.)
+// SHIFT: rows that begin and end anywhere.  Packs are those of memory; the elements before the row's first and behind its last, fewer than a pack each, go
+// to threads one by one, beside their packs.  The weight's packs lie otherwise: a block takes every G-th row, G a multiple of a pack's elements, so that
+// it is put in place once, in shared memory.  (7,000 rows of 8,191 in bf16 with norm and sum, element by element 317 us; with first and last packs that are
+// checked element by element, as part of every pack's code, and the weight's packs shifted anew for each row 273, put in place once 128, so 102.  Rows that
+// begin at packs lose by keeping the weight: 74 us and 82.)
 template <typename T, int kEach, int TPR, int MOST, bool NORM, bool SHIFT>
 __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_rows(RowArgs a) {
     constexpr bool kBlock = TPR == 0;
@@ -162,9 +153,15 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
     const int lane = kBlock ? threadIdx.x : threadIdx.x % kPart, lane32 = threadIdx.x & 31, warps = blockDim.x >> 5;
     const T* w = NORM ? static_cast<const T*>(a.weight) : nullptr;
     const long long first = kBlock ? blockIdx.x : (long long)blockIdx.x * (MOST / kPart) + threadIdx.x / kPart, step = kBlock ? gridDim.x : (long long)gridDim.x * (MOST / kPart);
-    // elements of a row's first pack that lie before the row
-    const int shift = SHIFT ? (int)(reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + first * a.x_stride) / sizeof(T)) & (VEC - 1) : 0;
-    auto begin = [&](int j) { return (j * each_row + lane) * VEC - shift; };   // of this thread's pack j in the row
+    // the row's first pack begins at `head`, behind `packs` of them lie `tail` elements
+    const int away = SHIFT ? (int)(reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + first * a.x_stride) / sizeof(T)) & (VEC - 1) : 0;
+    const int head = SHIFT ? min((VEC - away) & (VEC - 1), a.dim) : 0, packs = (a.dim - head) / VEC, tail = a.dim - head - packs * VEC;
+    auto begin = [&](int j) { return head + (j * each_row + lane) * VEC; };    // of this thread's pack j in the row
+    constexpr int kSingle = !SHIFT ? 0 : kBlock || TPR >= 2 * VEC ? 1 : 2 * VEC / (TPR ? TPR : 1);
+    auto single = [&](int q, int of) {                                          // element of thread `of` beside its packs; -1: none
+        const int i = of + q * (kBlock ? 0 : kPart);
+        return i < VEC ? (i < head ? i : -1) : i < VEC + tail ? head + packs * VEC + i - VEC : -1;
+    };
     if (kBlock && threadIdx.x == 0) s_tops64[0] = 0;
     extern __shared__ uint4 s_weight[];   // kKeep: the weight's packs of each thread
     if (kKeep)
@@ -172,16 +169,24 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
         for (int j = 0; j < NV; ++j) {
             P p;
             p.ones();
-            if (w && begin(j) < a.dim) p.read_each(w, begin(j), a.dim);
+            if (w && begin(j) + VEC <= a.dim) p.read_each(w, begin(j));
             s_weight[j * blockDim.x + threadIdx.x] = make_uint4(p.word[0], p.word[1], p.word[2], p.word[3]);
         }
+    float alone_w[kSingle + 1];   // the weight of the elements beside the packs
+#pragma unroll
+    for (int q = 0; q < kSingle; ++q) {
+        const int i = single(q, lane);
+        alone_w[q] = NORM && w && i >= 0 ? to_float(w[i]) : 1.f;
+    }
+    auto weighed = [&](int q, float v) { return NORM ? v * alone_w[q] : v; };
     int turn = 0;
     long long row = first;
     // (a part of a warp whose rows have ended stays for the others)
     do {
     const bool live = row < a.n;
-    const int dim = live ? a.dim : 0;
+    const int dim = live ? a.dim : 0;   // (no pack of a row that is none)
     unsigned long long h[kEach / 2];   // the row, or its sum with the residual, two elements each
+    float alone[kSingle + 1];          // and the elements beside its packs
     float mine = 0.f, sum = 0.f;
     {
         const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
@@ -192,32 +197,27 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
             px[j].zeros();
             if (NORM) { pr[j].zeros(); pw[j].ones(); }
             const int at = begin(j);
-            if (at < dim) {
+            if (at + VEC <= dim) {
+                px[j].read(x, at);
+                if (NORM && r) pr[j].read(r, at);
                 if (NORM && !kKeep && w) pw[j].read(w, at);
-                if (!SHIFT || (at >= 0 && at + VEC <= dim) || (kKeep && (row > 0 || at >= 0) && (row < a.n - 1 || at + VEC <= dim))) {
-                    px[j].read(x, at);
-                    if (NORM && r) pr[j].read(r, at);
-                } else {
-                    px[j].read_each(x, at, dim);
-                    if (NORM && r) pr[j].read_each(r, at, dim);
-                }
             }
+        }
+#pragma unroll
+        for (int q = 0; q < kSingle; ++q) {
+            const int i = live ? single(q, lane) : -1;
+            alone[q] = i >= 0 ? to_float(x[i]) : 0.f;
+            if (NORM && r && i >= 0) alone[q] += to_float(r[i]);
         }
         unsigned long long sums = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int at = begin(j);
-            const bool edge = kKeep && (at < 0 || at + VEC > dim);
             if (kKeep) pw[j].set(s_weight[j * blockDim.x + threadIdx.x]);
 #pragma unroll
             for (int e = 0; e < VEC; e += 2) {
                 const int i = (j * VEC + e) / 2;
                 h[i] = pair(px[j].get(e), px[j].get(e + 1));
                 if (NORM && r) h[i] = add2(h[i], pair(pr[j].get(e), pr[j].get(e + 1)));
-                if (edge) {
-                    const float2 v = halves(h[i]);
-                    h[i] = pair((unsigned)(at + e) < (unsigned)dim ? v.x : 0.f, (unsigned)(at + e + 1) < (unsigned)dim ? v.y : 0.f);
-                }
                 if (NORM) sums = fma2(h[i], h[i], sums);
                 const float2 u = halves(NORM ? mul2(h[i], pair(pw[j].get(e), pw[j].get(e + 1))) : h[i]);
                 mine = larger(larger(mine, u.x), u.y);
@@ -225,6 +225,11 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
         }
         const float2 s = halves(sums);
         sum = s.x + s.y;
+#pragma unroll
+        for (int q = 0; q < kSingle; ++q) {
+            if (NORM) sum = fmaf(alone[q], alone[q], sum);
+            mine = larger(mine, weighed(q, alone[q]));
+        }
     }
     float top32 = kPart == 32 ? warp_larger(mine) : lanes_reduce<kPart>(mine, LargerOp());
     if (NORM) sum = lanes_reduce<kPart>(sum, SumOp());
@@ -241,31 +246,42 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
         bool some = false;
 #pragma unroll
         for (int i = 0; i < kEach / 2; ++i) { const float2 v = halves(h[i]); some = some || v.x != 0.f || v.y != 0.f; }
+#pragma unroll
+        for (int q = 0; q < kSingle; ++q) some = some || alone[q] != 0.f;
         some = kBlock ? __syncthreads_or(some) : lanes_reduce<kPart>((int)some, MaxOp());
         if (top32 == 0.f && !some) wild = false;
     }
 
-    // For each lane of the warp that needs it: f(lane, its row, element of the row, its value in 32 bits, its sum and value in 64), an element
-    // of that lane's for each of the 32 (an element < 0: none).
+    // For each lane of the warp that needs it: f(lane, its row, element of the row, its value in 32 bits, its sum and value in 64), an element of that
+    // lane's packs for each of the 32 (an element < 0: none), and then those beside its packs.
     auto together = [&](bool need, auto&& f) {
         __syncwarp();   // what f writes lies over what its lane wrote, what it reads under what that writes next
         for (unsigned todo = __ballot_sync(0xffffffffu, need && live); todo; todo &= todo - 1) {
             const int whose = __ffs(todo) - 1;
             const long long of = __shfl_sync(0xffffffffu, row, whose);
-            const int l = kBlock ? (int)(threadIdx.x & ~31u) + whose : whose % kPart;
-            int i = (lane32 / VEC * each_row + l) * VEC + lane32 % VEC - (SHIFT ? __shfl_sync(0xffffffffu, shift, whose) : 0);
-            if (lane32 >= kEach || i >= a.dim) i = -1;
-            float v = 0.f;
-            double s64 = 0, v64 = 0;
-            if (i >= 0) {
-                const float x = to_float(static_cast<const T*>(a.x)[of * a.x_stride + i]);
-                const float r = NORM && a.residual ? to_float(static_cast<const T*>(a.residual)[of * a.residual_stride + i]) : 0.f;
-                const float by = NORM && w ? to_float(w[i]) : 1.f;
-                v = NORM ? (x + r) * by : x;
-                s64 = (double)x + (double)r;
-                v64 = s64 * (double)by;
+            const int l = kBlock ? (int)(threadIdx.x & ~31u) + whose : whose % kPart, first_pack = SHIFT ? __shfl_sync(0xffffffffu, head, whose) : 0;
+            int i = first_pack + (lane32 / VEC * each_row + l) * VEC + lane32 % VEC, beside = -1;
+            if (lane32 >= kEach || i - lane32 % VEC + VEC > a.dim) i = -1;
+#pragma unroll
+            for (int q = 0; q < kSingle; ++q) {
+                const int e = __shfl_sync(0xffffffffu, single(q, lane), whose);
+                if (lane32 == q) beside = e;
             }
-            f(whose, of, i, v, s64, v64);
+#pragma unroll 1
+            for (int turn = 0; turn < (SHIFT ? 2 : 1); ++turn) {
+                if (SHIFT && turn) i = beside;
+                float v = 0.f;
+                double s64 = 0, v64 = 0;
+                if (i >= 0) {
+                    const float x = to_float(static_cast<const T*>(a.x)[of * a.x_stride + i]);
+                    const float r = NORM && a.residual ? to_float(static_cast<const T*>(a.residual)[of * a.residual_stride + i]) : 0.f;
+                    const float by = NORM && w ? to_float(w[i]) : 1.f;
+                    v = NORM ? (x + r) * by : x;
+                    s64 = (double)x + (double)r;
+                    v64 = s64 * (double)by;
+                }
+                f(whose, of, i, v, s64, v64);
+            }
         }
         __syncwarp();
     };
@@ -279,7 +295,7 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
         P pw;
         if (NORM) pw.ones();
         if (kKeep) pw.set(s_weight[j * blockDim.x + threadIdx.x]);
-        else if (NORM && w && begin(j) < dim) pw.read_again(w, begin(j));
+        else if (NORM && w && begin(j) + VEC <= dim) pw.read_again(w, begin(j));
 #pragma unroll
         for (int e = 0; e < VEC; e += 2) {
             const int i = (j * VEC + e) / 2;
@@ -295,16 +311,22 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int at = begin(j);
-        if (at >= dim) continue;
+        if (at + VEC > dim) continue;
         const unsigned* v = c + j * VEC;
-        if (!SHIFT || (at >= 0 && at + VEC <= dim && (reinterpret_cast<uintptr_t>(out + at) & (VEC - 1)) == 0)) {
+        if (!SHIFT || (reinterpret_cast<uintptr_t>(out + at) & (VEC - 1)) == 0) {
             if constexpr (VEC == 8) *reinterpret_cast<uint2*>(out + at) = make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7]));
             else *reinterpret_cast<unsigned*>(out + at) = four(v[0], v[1], v[2], v[3]);
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (at + e >= 0 && at + e < dim) out[at + e] = (signed char)v[e];
+            for (int e = 0; e < VEC; ++e) out[at + e] = (signed char)v[e];
         }
+    }
+#pragma unroll
+    for (int q = 0; q < kSingle; ++q) {
+        const int i = live ? single(q, lane) : -1;
+        const float u = weighed(q, alone[q]), m = fmaf(u, inverse, kRint);
+        off = fmaxf(off, fabsf(fmaf(u, inverse, kRint - m)));
+        if (i >= 0) out[i] = (signed char)__float_as_uint(m);
     }
     const bool unsure = wild || off > kNearTie<NORM>;
     float scale = !(top32 > 0) ? 0.f : NORM ? top32 / (127.f * sqrtf(sum / (float)a.dim + a.eps)) : top32 / 127.f;
@@ -318,7 +340,7 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
                 const bool all = __shfl_sync(0xffffffffu, (int)wild, whose);
                 const float least = __shfl_sync(0xffffffffu, near, whose);
                 const unsigned long long m = lanes_reduce<32>(all || fabsf(v) >= least ? magnitude(v64) : 0ull, MaxOp());
-                if (lane32 == whose) t = m;
+                if (lane32 == whose) t = max(t, m);
             });
             if constexpr (!kBlock) t = lanes_reduce<kPart>(t, MaxOp());
             else {
@@ -334,7 +356,7 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
             if (NORM) {
                 together(wild, [&](int whose, long long, int, float, double s64, double) {
                     const double m = lanes_reduce<32>(s64 * s64, SumOp());
-                    if (lane32 == whose) s = m;
+                    if (lane32 == whose) s += m;
                 });
                 s = lanes_reduce<kPart>(s, SumOp());
                 if constexpr (kBlock) {
@@ -359,7 +381,10 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_r
         T* to = static_cast<T*>(a.sum) + (live ? row : 0) * a.sum_stride;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (begin(j) < dim) P::template write<SHIFT>(to, begin(j), dim, h + j * (VEC / 2));
+            if (begin(j) + VEC <= dim) P::write(to + begin(j), h + j * (VEC / 2));
+#pragma unroll
+        for (int q = 0; q < kSingle; ++q)
+            if (live && single(q, lane) >= 0) to[single(q, lane)] = from_float<T>(alone[q]);
     }
     if (live && lane == 0) a.scales[row] = scale;
     row += step;
@@ -425,11 +450,11 @@ psb_status start(const RowArgs& a, int threads, int sms, cudaStream_t s) {
 template <typename T, bool NORM, bool SHIFT>
 psb_status by_length(const RowArgs& a, int sms, cudaStream_t s) {
     constexpr int VEC = Pack<T>::VEC, kMost = VEC == 8 ? 32 : 16;
-    const int span = a.dim + (SHIFT ? VEC - 1 : 0);
+    const int span = a.dim;
     auto warps = [&](int each) { return ((span + each - 1) / each + 31) / 32 * 32; };   // threads, in whole warps
     if (span > 512 && a.n * (long long)warps(kMost) < 1024ll * sms && warps(16) <= 1024) {
         int threads = warps(16);
-        while (threads <= 512 && threads < warps(VEC) && a.n * (long long)threads < 1024ll * sms) threads *= 2;
+        while (threads <= 512 && threads < warps(VEC) && a.n * (long long)threads * 2 <= 1024ll * sms) threads *= 2;   // (all rows at once)
         return start<T, 16, 0, 1024, NORM, SHIFT>(a, std::min(threads, warps(VEC)), sms, s);
     }
     if (span <= 4 * 16) return start<T, 16, 4, 256, NORM, SHIFT>(a, 0, sms, s);
@@ -451,7 +476,7 @@ psb_status by_layout(const RowArgs& a, int sms, cudaStream_t s) {
     // the rows' arrays begin at the same place of a pack in every row
     auto as_rows = [&](const void* p, long long stride) { return !p || (place(p, e) == at && (int)(stride & (VEC - 1)) == step); };
     const bool packs = as_rows(a.residual, a.residual_stride) && as_rows(a.sum, a.sum_stride) && place(a.weight, e) == 0;
-    if (packs && a.dim + VEC - 1 <= 1024 * (VEC == 8 ? 32 : 16)) {
+    if (packs && a.dim <= 1024 * (VEC == 8 ? 32 : 16)) {
         const bool plain = at == 0 && step == 0 && a.dim % VEC == 0 && place(a.codes, 1) == 0 && (a.code_stride & (VEC - 1)) == 0;
         return plain ? by_length<T, NORM, false>(a, sms, s) : by_length<T, NORM, true>(a, sms, s);
     }
