@@ -475,7 +475,8 @@ psb_status select(SelectArgs a, int batch, int sms, cudaStream_t s) {
     a.per_beam = std::max(1, warps / a.beams);
     a.by_beam = (unsigned)(((1ull << 32) + a.per_beam - 1) / a.per_beam);
     a.groups = 32;
-    while (a.groups > 1 && a.per_beam * a.beams * a.groups > kMaxGroups) a.groups /= 2;
+    // (about 32 k of them make the bound tight enough, and up to kThreads are counted at once)
+    while (a.groups > 1 && (a.per_beam * a.beams * a.groups > kMaxGroups || a.per_beam * a.beams * a.groups / 2 >= 32 * a.k)) a.groups /= 2;
     const void* kernel = reinterpret_cast<const void*>(k_beam_select<T>);
     PSB_TRY(kernel_shared(kernel, sizeof(SelectShared)));
     if (blocks > 8) {   // clusters of more than 8 are asked for once a device
