@@ -682,7 +682,7 @@ psb_status psb_beam_select(const void* d_logits, int type, int64_t row_stride, c
 /* States [layers][batch][beams][heads][tokens][token_bytes] brought into the new order: out[.., item, j, ..] = in[.., item, parent[item][j], ..]
  * for the first d_lengths[item] tokens (NULL: all); what lies behind them is left as it was, and so is a beam whose parent is outside
  * 0..beams-1.  d_out is d_in (any parents: the states are reordered where they are) or does not overlap it.  d_parents [batch][beams];
- * beams <= 64; layers * batch <= 65,535. */
+ * beams <= 64; batch and layers <= 65,535. */
 psb_status psb_beam_reorder(const void* d_in, void* d_out, const int* d_parents, int layers, int batch, int beams, int heads, int tokens,
                             int64_t token_bytes, const int* d_lengths, int device, void* stream);
 

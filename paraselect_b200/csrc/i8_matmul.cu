@@ -37,6 +37,9 @@ constexpr int kThreads = 32 * kEpilogue + 64;   // one warp loads, one issues pr
 constexpr int kMaxStages = 12;
 constexpr int kMaxParts = 8;               // blocks that share a tile
 constexpr int kRing = 200 * 1024;
+// More than half of an SM's shared memory, so that no two blocks of these kernels share an SM: blocks of a cluster hold their tensor memory while they wait for
+// one another, and two clusters, each with a block that waits for the tensor memory that the other's holds, would wait for good.
+constexpr size_t kAlone = 116 * 1024;
 constexpr int kWaitPolls = 1 << 22;
 constexpr long long kAllTiles = 0x7fffffffffffffffll;
 
@@ -670,7 +673,7 @@ psb_status run_pairs(MatmulArgs a, int sms, cudaStream_t s) {
     a.slabs = (a.k + kSlab - 1) / kSlab;
     const int stage_bytes = (kChannels + a.tokens / 2) * kSlab;
     a.stages = std::min(kMaxStages, kRing / stage_bytes);
-    const size_t smem = 1024 + (size_t)a.stages * stage_bytes;
+    const size_t smem = std::max(kAlone, 1024 + (size_t)a.stages * stage_bytes);
     CUtensorMap map_w, map_x;
     PSB_TRY(codes_map(&map_w, a.w, a.n, a.k, a.w_stride, kChannels));
     PSB_TRY(codes_map(&map_x, a.x, a.m, a.k, a.x_stride, a.tokens / 2));
@@ -689,25 +692,28 @@ psb_status run_pairs(MatmulArgs a, int sms, cudaStream_t s) {
 
 template <typename T>
 psb_status run(MatmulArgs a, int sms, cudaStream_t s) {
-    // (k = 4,096, by dp4a and on the tensor cores: 1 token and 32,000 channels 21.7 and 25.7 us, 4,096 channels 5.9 and 7.1; 4 tokens and 32,000
-    // channels 30.4 and 26.5, 4,096 channels 5.4 and 7.4)
+    // By dp4a and on the tensor cores, k = 4,096: 1 token and 32,000 channels 21.6 and 25.7 us, 4,096 channels 4.2 to 5.4 and 7.1; 2 tokens 28.3 and 26.6, 5.3 and 7.1; 4 tokens
+    // 30.4 and 26.5, 5.1 and 7.2.  Short rows: 2 tokens x 200,000 x 64 6.1 and 11.2; 4 x 200,000 x 64 7.3 and 10.6, 4 x 135,872 x 264 29 and 16.6.
     const bool few = a.m == 1 || (a.m <= kFewTokens && (a.n <= kChannels * (sms / 2) || a.k <= kFewDepth));
     if (few && a.issued == kAllTiles) return run_few<T>(a, sms, s);
-    // tiles of tokens of even size, each a multiple of 16: of 256 at most, or of 128 where they would not fill half of the GPU
+    // tiles of tokens of even size, each a multiple of 16: of 256 at most, or of 128 where they would not fill half of the GPU (512 x 4,096 x 4,096: 17.9 and 16.2 us,
+    // 609 x 641 x 797: 12.1 and 9.8)
     a.channel_tiles = (a.n + kChannels - 1) / kChannels;
     int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
     if (token_tiles > 1 && (long long)token_tiles * a.channel_tiles * 2 < sms) token_tiles = (a.m + 127) / 128;
     a.tokens = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
     const long long tiles = (long long)token_tiles * a.channel_tiles;
+    // Pairs and single blocks: 1,024 x 32,000 x 4,096 96.9 and 122.8 us, 256 x 14,336 x 4,096 19.5 and 20.9, 200 x 32,000 x 4,096 32.1 and 33.6, 1,024 x 4,096 x 4,096 17.9 and 18.5
     if (a.m >= kPairMin && tiles * 2 >= sms) return run_pairs<T>(a, sms, s);
     if (tiles > 0x3fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^30 - 1 tiles of 128 x 256 outputs");
     a.tiles = (int)tiles;
     a.slabs = (a.k + kSlab - 1) / kSlab;
+    // blocks that share a tile: while the GPU has room for twice as many, and each two slabs or more (256 x 4,096 x 14,336: 4 blocks 23.4 us, 2 with tiles of 128 tokens 33)
     int parts = 1;
     while (parts < kMaxParts && tiles * parts * 2 <= sms && a.slabs >= parts * 4) parts *= 2;
     const int stage_bytes = (kChannels + a.tokens) * kSlab;
     a.stages = std::min(std::min(kMaxStages, std::max(2, (a.slabs + parts - 1) / parts)), kRing / stage_bytes);
-    const size_t smem = 1024 + std::max((size_t)a.stages * stage_bytes, parts > 1 ? (size_t)a.tokens * kChannels * 4 : 0);
+    const size_t smem = std::max(kAlone, 1024 + std::max((size_t)a.stages * stage_bytes, parts > 1 ? (size_t)a.tokens * kChannels * 4 : 0));
     CUtensorMap map_w, map_x;
     PSB_TRY(codes_map(&map_w, a.w, a.n, a.k, a.w_stride, kChannels));
     PSB_TRY(codes_map(&map_x, a.x, a.m, a.k, a.x_stride, a.tokens));

@@ -162,7 +162,7 @@ def reordered(states, parents, lengths, into):
 
 
 @pytest.mark.parametrize("layers,batch,beams,heads,tokens,bytes_", [(1, 1, 1, 1, 1, 1), (2, 3, 4, 2, 5, 32), (1, 2, 5, 3, 17, 6), (3, 1, 8, 8, 33, 128), (1, 2, 9, 2, 10, 20), (2, 2, 16, 1, 7, 256),
-                                                                    (1, 1, 64, 2, 9, 48), (1, 3, 33, 1, 11, 7), (2, 5, 4, 8, 515, 128), (1, 1, 2, 1, 100000, 160)])
+                                                                    (1, 1, 64, 2, 9, 48), (1, 3, 33, 1, 11, 7), (2, 5, 4, 8, 515, 128), (1, 1, 2, 1, 100000, 160), (300, 250, 2, 1, 2, 16)])
 @pytest.mark.parametrize("place", [True, False])
 @pytest.mark.parametrize("ragged", [True, False])
 def test_reorder(psb, layers, batch, beams, heads, tokens, bytes_, place, ragged):

@@ -136,3 +136,19 @@ def test_two_streams_and_graphs(psb, m, n, k):
             g.replay()
     for x, xs, w, ws, out in sets:
         assert close(out, expected(x, xs, w, ws, k), torch.float32)
+
+
+def test_many_streams_of_split_paired_and_single_products(psb):
+    """Calls of every kernel under way together on eight streams, small rings and large: their blocks hold tensor memory while they wait for each other."""
+    shapes = [(16, 300, 1100), (224, 30000, 256), (256, 9000, 128), (40, 700, 4096), (100, 513, 2048), (1, 4000, 4096), (200, 20000, 100), (30, 128, 9000)]
+    calls = []
+    for i, (m, n, k) in enumerate(shapes):
+        x, w, xs, ws = codes(m, k, 50 + i), codes(n, k, 60 + i), scales(m, 70 + i, 1.0), scales(n, 80 + i, 1e-4)
+        calls.append((torch.cuda.Stream(), x, xs, w, ws, torch.zeros((m, n), device="cuda"), m, n, k))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, x, xs, w, ws, out, m, n, k in calls:
+            psb.i8_matmul(x, xs, m, w, ws, n, k, out, x_stride=x.stride(0), w_stride=w.stride(0), stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for s, x, xs, w, ws, out, m, n, k in calls:
+        assert close(out, expected(x, xs, w, ws, k), torch.float32)

@@ -71,6 +71,24 @@ def test_norm(psb, t, n, dim, residual, weight):
     assert torch.equal(total, (x.float() + (r.float() if residual else 0)).to(t))
 
 
+# enough rows to fill the GPU, at both sides of every change in the threads a row and in the elements a thread, rows that begin at packs and that do not
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n,dim", [(40000, 1), (40001, 17), (40000, 64), (40003, 65), (30000, 128), (30000, 129), (20001, 256), (20000, 263), (9001, 512), (9000, 519), (5000, 1024), (5003, 1031),
+                                   (3000, 4096), (3001, 4101), (1300, 8192), (1301, 8193), (1200, 9216), (1203, 9221), (700, 16384), (701, 16391), (600, 32768)])
+def test_many_rows(psb, t, n, dim):
+    x, r, w = values(n, dim, t, n), values(n, dim, t, n + 1), (1 + 0.2 * torch.randn(dim, device="cuda")).to(t)
+    codes, scales = torch.empty((n, dim), dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda")
+    psb.i8_encode_rows(x, n, dim, codes, scales)
+    want, scale = expected(x)
+    assert torch.equal(codes, want)
+    check_scales(scales, scale)
+    want, scale = expected(x, r, w, float(np.float32(1e-5)))
+    total = (x.float() + r.float()).to(t)
+    psb.i8_norm_rows(x, n, dim, w, 1e-5, codes, scales, d_residual=r, d_sum=r)
+    assert torch.equal(codes, want) and torch.equal(r, total)
+    check_scales(scales, scale)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("dim,pads", [(96, (3, 5, 7, 9)), (96, (8, 16, 24, 32)), (1000, (0, 1, 0, 0)), (4096, (8, 8, 8, 16)), (50, (1, 1, 1, 1))])
 @pytest.mark.parametrize("where", ["apart", "rows", "residual"])
