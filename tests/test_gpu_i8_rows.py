@@ -56,7 +56,7 @@ def test_encode(psb, t, n, dim):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("n,dim", [(1, 1), (3, 8), (700, 64), (50, 100), (33, 127), (5, 1024), (3, 1031), (300, 4096), (2, 5003), (1, 8192), (5, 8192), (2, 16384), (1, 20001), (1, 40000)])
+@pytest.mark.parametrize("n,dim", [(1, 1), (3, 8), (700, 64), (50, 100), (33, 127), (5, 1024), (3, 1031), (300, 4096), (2, 5003), (1, 8192), (5, 8192), (2, 16384), (1, 20001), (1, 40000), (3, 53248), (2, 131064), (1, 131071)])
 @pytest.mark.parametrize("residual,weight", [(True, True), (False, True), (True, False)])
 def test_norm(psb, t, n, dim, residual, weight):
     x = values(n, dim, t, n + dim)
