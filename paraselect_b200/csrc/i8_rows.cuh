@@ -126,11 +126,15 @@ __device__ __forceinline__ float warp_larger(float v) {
 }
 
 // Blocks of MOST threads that an SM's registers shall hold.
-template <int kEach, int MOST, bool NORM> constexpr int blocks_of() { return MOST == 256 ? (kEach == 32 ? (NORM ? 3 : 4) : (NORM ? 4 : 6)) : MOST == 288 ? 2 : 1; }
+// (16,384 x 8,192 bf16 with norm: 3 170 us, 4 164, 5 216; rows that begin anywhere, 200,000 x 500: 3 141, 4 160; 30,000 x 4,096 without: 4 68, 5 64.5, 6 63; fp32,
+// 100,000 x 1,000 with norm: 4 189, 5 225; 1M x 96 without: 6 74, 7 70; 100,000 x 333: 6 34, 7 38; blocks of 512, 8,000 x 16,384 bf16 with norm: 1 235, 2 181, without 125 and 85)
+template <int kEach, int MOST, bool NORM, bool SHIFT> constexpr int blocks_of() {
+    return MOST == 256 ? (kEach == 32 ? (NORM ? (SHIFT ? 3 : 4) : 6) : NORM ? 4 : SHIFT ? 6 : 7) : MOST == 288 || (MOST == 512 && !(NORM && SHIFT)) ? 2 : 1;
+}
 
-// One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in packs of 16 bytes.  What few elements need - 64 bits next to ties,
-// at the top, in rows out of fp32's range - is read again from memory, before the sum is written, by the 32 lanes of a warp for the one that found
-// it.  Code for it beside every element took five times the kernel's time, and a thread of its own for it half of the rest, the block waiting
+// One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in
+// packs of 16 bytes.  What few elements need - 64 bits next to ties, at the top, in rows out of fp32's range - is read again from memory, before the sum
+// is written, by the 32 lanes of a warp for the one that found it.  Code for it beside every element took five times the kernel's time, and a thread of its own for it half of the rest, the block waiting
 // (16,384 rows of 8,192 in bf16: 789 and 499 us).  fp32 arithmetic goes two elements an instruction: the kernel was bound by issue (239 us).
 //
 // SHIFT: rows that begin and end anywhere.  Packs are those of memory; the elements before the row's first and behind its last, fewer than a pack each, go
@@ -139,7 +143,7 @@ template <int kEach, int MOST, bool NORM> constexpr int blocks_of() { return MOS
 // checked element by element, as part of every pack's code, and the weight's packs shifted anew for each row 273, put in place once 128, so 102.  Rows that
 // begin at packs lose by keeping the weight: 74 us and 82.)
 template <typename T, int kEach, int TPR, int MOST, bool NORM, bool SHIFT>
-__global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM>())) k_i8_rows(RowArgs a) {
+__global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM, SHIFT>())) k_i8_rows(RowArgs a) {
     constexpr bool kBlock = TPR == 0;
     constexpr int kPart = kBlock ? 32 : TPR;   // threads that exchange by shuffles
     const int each_row = kBlock ? (int)blockDim.x : TPR;
@@ -533,7 +537,7 @@ psb_status start(const RowArgs& a, int threads, int sms, cudaStream_t s) {
     const long long rows = TPR ? MOST / (TPR ? TPR : 1) : 1, blocks = (a.n + rows - 1) / rows;
     long long grid = blocks;
     if (NORM && SHIFT) {   // as many blocks as fit, of as many rows each as the others, a multiple of a pack's elements
-        const long long fit = (long long)sms * std::max(1, blocks_of<kEach, MOST, NORM>() * MOST / threads), turns = (blocks + fit - 1) / fit;
+        const long long fit = (long long)sms * std::max(1, blocks_of<kEach, MOST, NORM, SHIFT>() * MOST / threads), turns = (blocks + fit - 1) / fit;
         grid = (blocks + turns - 1) / turns;
         if (grid < blocks) grid = std::min(blocks, std::max(8ll, std::min((grid + 7) / 8 * 8, fit / 8 * 8)));
     }
