@@ -140,6 +140,11 @@ __device__ __forceinline__ void store_tile(const MatmulArgs& a, float* scales, c
     }
 }
 
+// Where a block gave up, the copies that are under way to its ring land before it ends.  For one thread.
+__device__ __forceinline__ void await_loads(uint64_t* full, int loads, int stages, int polls) {
+    for (int i = max(0, loads - stages); i < loads; ++i) tc::mbar_wait(&full[i % stages], (i / stages) & 1, polls);
+}
+
 // SPLIT: the blocks of a cluster share a tile, each with its share of the slabs.  Otherwise a block takes every gridDim.x-th tile, its
 // accumulators in two buffers, so that the epilogue of one tile lies beside the products of the next.
 template <typename T, bool SPLIT>
@@ -147,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], ready[2], drained[2], last;
     __shared__ uint32_t tmem_at;
-    __shared__ int gave_up;
+    __shared__ int gave_up, loads;
     __shared__ __align__(16) float s_scales[2][kMaxTokens];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -196,10 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
                     tc::tma_load_2d(to + kChannels * kSlab, &map_x, slab * kSlab, t0, &full[st]);
                 }
             }
-            if (!ok) {   // the loads under way land before the block ends
-                gave_up = 1;
-                for (int i = max(0, at - a.stages); i < at; ++i) tc::mbar_wait(&full[i % a.stages], (i / a.stages) & 1, a.polls);
-            }
+            loads = at;
+            if (!ok) gave_up = 1;
         }
         __syncwarp();
     } else if (warp == kEpilogue + 1) {
@@ -273,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     __syncthreads();
     tc::tc_fence_after();
     if (warp == kEpilogue + 1) tc::tmem_dealloc(tmem, tmem_columns(a.tokens, kBuffers));
+    if (gave_up && threadIdx.x == 0) await_loads(full, loads, a.stages, a.polls);
 
     if constexpr (SPLIT) {
         cg::cluster_group cluster = cg::this_cluster();
@@ -362,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], ready[2], drained[2], last;
     __shared__ uint32_t tmem_at;
-    __shared__ int gave_up;
+    __shared__ int gave_up, loads;
     __shared__ __align__(16) float s_scales[2][kMaxTokens];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     cg::cluster_group cluster = cg::this_cluster();
@@ -402,11 +406,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
                     pair_load(to + kChannels * kSlab, &map_x, slab * kSlab, t0 + rank * mine, in_first(&full[st]));
                 }
             }
-            if (!ok) {   // the loads under way land before the block ends (the second block's count here too, and are older than its wait that gave up)
-                gave_up = 1;
-                if (rank == 0)
-                    for (int i = max(0, at - a.stages); i < at; ++i) tc::mbar_wait(&full[i % a.stages], (i / a.stages) & 1, a.polls);
-            }
+            loads = at;
+            if (!ok) gave_up = 1;
         }
         __syncwarp();
     } else if (warp == kEpilogue + 1) {
@@ -467,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
     tc::tc_fence_after();
     if (warp == kEpilogue + 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
     const int lost = gave_up | *cluster.map_shared_rank(&gave_up, rank ^ 1);
+    if (lost && rank == 0 && threadIdx.x == 0) await_loads(full, loads, a.stages, a.polls);   // (both blocks' copies count here)
     cluster.sync();   // neither block ends while the other looks
     if (lost) {
         for (int tile = first; tile < a.tiles; tile += step) {
