@@ -675,14 +675,14 @@ psb_status psb_i8_matmul_limited(const int8_t* d_x, int64_t x_stride, const floa
 /* The k best continuations of each of `batch` items over its beams and the vocabulary: total = d_scores[item][beam] + log p(token), log p the
  * log-softmax of the beam's logits (d_logits [batch * beams][row_stride] of `type`), largest first, ties to the lowest (beam, token).  A token
  * with logit -inf is never chosen; neither is one of a beam whose score is not finite or whose logits hold a NaN or +inf or nothing but -inf.
- * d_parents, d_tokens [batch][k] int32 (-1 where fewer are left), d_totals [batch][k] fp32 (-inf there).  beams <= 64, k <= 64,
- * vocab <= 2^24, batch <= 2^20. */
+ * d_parents, d_tokens [batch][k] int32 (-1 where fewer are left), d_totals [batch][k] fp32 (-inf there).  d_totals may be
+ * d_scores itself where k = beams; no other output lies over another array.  beams <= 64, k <= 64, vocab <= 2^24, batch <= 2^20. */
 psb_status psb_beam_select(const void* d_logits, int type, int64_t row_stride, const float* d_scores, int batch, int beams, int vocab, int k,
                            int* d_parents, int* d_tokens, float* d_totals, int device, void* stream);
 /* States [layers][batch][beams][heads][tokens][token_bytes] brought into the new order: out[.., item, j, ..] = in[.., item, parent[item][j], ..]
  * for the first d_lengths[item] tokens (NULL: all); what lies behind them is left as it was, and so is a beam whose parent is outside
- * 0..beams-1.  d_out is d_in (any parents: the states are reordered where they are) or does not overlap it.  d_parents [batch][beams];
- * beams <= 64; batch and layers <= 65,535. */
+ * 0..beams-1.  d_out is d_in (any parents: the states are reordered where they are) or does not overlap it, nor the parents and
+ * lengths.  d_parents [batch][beams]; beams <= 64; batch and layers <= 65,535. */
 psb_status psb_beam_reorder(const void* d_in, void* d_out, const int* d_parents, int layers, int batch, int beams, int heads, int tokens,
                             int64_t token_bytes, const int* d_lengths, int device, void* stream);
 

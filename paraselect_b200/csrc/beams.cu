@@ -576,6 +576,14 @@ psb_status psb_beam_select(const void* d_logits, int type, int64_t row_stride, c
     auto at = [](const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; };
     if (!at(d_logits, type == PSB_TYPE_F32 ? 4 : 2) || !at(d_scores, 4) || !at(d_parents, 4) || !at(d_tokens, 4) || !at(d_totals, 4))
         return fail(PSB_INVALID_ARGUMENT, "beam selection: a pointer is not aligned to its elements");
+    // An item's blocks read its scores before they write, but other items' blocks may not have read theirs: in place an item's totals are its own scores.
+    const int64_t e = type == PSB_TYPE_F32 ? 4 : 2;
+    const Span logits(d_logits, (int64_t)batch * beams, vocab * e, row_stride * e), scores(d_scores, batch, 4 * beams, 4 * beams);
+    const Span parents(d_parents, batch, 4 * k, 4 * k), tokens(d_tokens, batch, 4 * k, 4 * k), totals(d_totals, batch, 4 * k, 4 * k);
+    const bool over_scores = totals.meets(scores) && !(d_totals == d_scores && k == beams);
+    if (over_scores || parents.meets(scores) || tokens.meets(scores) || parents.meets(logits) || tokens.meets(logits) || totals.meets(logits) || parents.meets(tokens) ||
+        parents.meets(totals) || tokens.meets(totals))
+        return fail(PSB_INVALID_ARGUMENT, "beam selection: an output lies over another array (the totals may be the scores themselves where k is the number of beams)");
     DeviceScope on;
     PSB_TRY(on.enter(device));
     SelectArgs a{};
@@ -602,6 +610,9 @@ psb_status psb_beam_reorder(const void* d_in, void* d_out, const int* d_parents,
     if (b0 != o0 && b0 < o0 + size && o0 < b0 + size) return fail(PSB_INVALID_ARGUMENT, "beam reordering: the buffers overlap without being the same");
     if (reinterpret_cast<uintptr_t>(d_parents) % 4 || reinterpret_cast<uintptr_t>(d_lengths) % 4)
         return fail(PSB_INVALID_ARGUMENT, "beam reordering: a pointer is not aligned to its elements");
+    const Span states(d_out, 1, size, 0);
+    if (states.meets(Span(d_parents, batch, 4 * beams, 4 * beams)) || states.meets(Span(d_lengths, d_lengths ? batch : 0, 4, 4)))
+        return fail(PSB_INVALID_ARGUMENT, "beam reordering: the states lie over the parents or the lengths");
     DeviceScope on;
     PSB_TRY(on.enter(device));
     ReorderArgs a{};

@@ -96,6 +96,14 @@ constexpr uint64_t KEY_MAX = ~0ull;
 psb_status kernel_shared(const void* kernel, size_t bytes);
 psb_status kernel_carveout_max(const void* kernel);
 
+// Bytes [begin, end) that `n` rows of `width` bytes span, `stride` bytes apart.
+struct Span {
+    uintptr_t begin, end;
+    Span(const void* p, int64_t n, size_t width, int64_t stride)
+        : begin(reinterpret_cast<uintptr_t>(p)), end(begin + (n > 0 ? (uintptr_t)(n - 1) * (uintptr_t)stride + width : 0)) {}
+    bool meets(const Span& o) const { return begin < o.end && o.begin < end; }
+};
+
 // Makes `device` current for a call and the one that was current before again at its end; `sms`: its multiprocessors.
 struct DeviceScope {
     int before = -1, sms = 0;

@@ -20,14 +20,6 @@ bool type_known(int type) { return type >= PSB_TYPE_F32 && type <= PSB_TYPE_BF16
 
 constexpr int kMaxRowDim = 131071;   // what psb_i8_matmul takes
 
-// Bytes [begin, end) that `n` rows of `width` bytes span, `stride` bytes apart.
-struct Span {
-    uintptr_t begin, end;
-    Span(const void* p, int64_t n, size_t width, int64_t stride)
-        : begin(reinterpret_cast<uintptr_t>(p)), end(begin + (n > 0 ? (uintptr_t)(n - 1) * (uintptr_t)stride + width : 0)) {}
-    bool meets(const Span& o) const { return begin < o.end && o.begin < end; }
-};
-
 psb_status check_rows(const void* d_rows, int type, int64_t n, int dim, int64_t row_stride, const int8_t* d_codes, int64_t code_stride, const float* d_scales) {
     if (!type_known(type)) return fail(PSB_INVALID_ARGUMENT, "the element type is none of PSB_TYPE_*");
     if (n < 0 || dim <= 0) return fail(PSB_INVALID_ARGUMENT, "rows to encode: a count below zero or rows without elements");

@@ -109,6 +109,15 @@ def test_ties(psb, t, vocab):
         check(psb, x, s, 20, row_stride=vocab + pad)
 
 
+@pytest.mark.parametrize("batch,beams,vocab", [(1, 4, 32000), (400, 3, 1000), (64, 8, 20000)])
+def test_totals_in_place_of_the_scores(psb, batch, beams, vocab):
+    logits, scores = make(batch, beams, vocab, torch.bfloat16, 91)
+    parents, tokens, totals = chosen(psb, logits, scores, beams)
+    p, t = torch.empty_like(parents), torch.empty_like(tokens)
+    psb.beam_select(logits, scores, batch, beams, vocab, beams, p, t, scores)
+    assert torch.equal(p, parents) and torch.equal(t, tokens) and torch.equal(scores, totals)
+
+
 @pytest.mark.parametrize("vocab", [5000, 128000])
 def test_sorted_and_concentrated_rows(psb, vocab):
     """The best tokens side by side, in one warp's share."""

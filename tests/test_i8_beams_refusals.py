@@ -80,6 +80,7 @@ def test_matmul_refusals():
 def test_select_refusals():
     logits, scores = torch.zeros((6, 10)), torch.zeros((2, 3))
     p, t, v = torch.zeros((2, 4), dtype=torch.int32), torch.zeros((2, 4), dtype=torch.int32), torch.zeros((2, 4))
+    many = torch.zeros(9)
     bad = lambda status, *a, **kw: refused(status, api.beam_select, *a, **kw)  # noqa: E731
     bad(1, logits, scores, -1, 3, 10, 4, p, t, v)
     bad(1, logits, scores, 2, 0, 10, 4, p, t, v)
@@ -88,6 +89,11 @@ def test_select_refusals():
     bad(1, logits, scores, 2, 3, 10, 4, p, t, v, row_stride=9)
     bad(1, logits, None, 2, 3, 10, 4, p, t, v)
     bad(1, logits.long(), scores, 2, 3, 10, 4, p, t, v)
+    for call in ((logits, scores, 2, 3, 10, 4, p, p, v),            # outputs over each other, over the logits, over the scores of other items
+                 (logits, scores, 2, 3, 10, 4, p, t, t.view(torch.float32)), (logits, scores, 2, 3, 10, 4, p, t, logits),
+                 (logits, scores, 2, 3, 10, 4, p, scores.view(torch.int32), v), (logits, scores, 2, 3, 10, 2, p, t, scores),
+                 (logits, many, 2, 3, 10, 3, p, t, many[1:])):
+        bad(1, *call)
     bad(2, logits, scores, 2, 65, 10, 4, p, t, v)
     bad(2, logits, scores, 2, 3, 10, 65, p, t, v)
     bad(2, logits, scores, 2, 3, (1 << 24) + 1, 4, p, t, v)
@@ -102,6 +108,8 @@ def test_reorder_refusals():
     bad(1, a, b, p, -1, 2, 3, 4, 5, 8)
     bad(1, a, b, None, 1, 2, 3, 4, 5, 8)
     bad(1, a, a[2:], p, 1, 2, 3, 4, 5, 8)                 # the buffers overlap without being the same
+    bad(1, a, b, b[6:].view(torch.int32), 1, 2, 3, 4, 5, 8)   # the parents, the lengths lie in the states
+    bad(1, a, b, p, 1, 2, 3, 4, 5, 8, d_lengths=b[-2:].view(torch.int32))
     bad(2, a, b, p, 1, 2, 65, 4, 5, 8)
     bad(2, a, b, p, 70000, 2, 3, 4, 5, 8)
     bad(2, a, b, p, 1, 2, 3, 4, 2**31 - 1, 1 << 40)
