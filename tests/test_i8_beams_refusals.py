@@ -115,6 +115,25 @@ def test_reorder_refusals():
     bad(2, a, b, p, 1, 2, 3, 4, 2**31 - 1, 1 << 40)
 
 
+def test_arrays_of_other_types():
+    """Codes are int8, scales and totals fp32, parents and tokens int32: anything else is not read as if it were."""
+    x, c, s, i = rows(), codes(), torch.zeros(4), torch.zeros((4, 4), dtype=torch.int32)
+    refused(1, api.i8_encode_rows, x, 4, 32, c.to(torch.uint8), s)
+    refused(1, api.i8_encode_rows, x, 4, 32, c, s.double())
+    refused(1, api.i8_norm_rows, x, 4, 32, None, 1e-5, c.int(), s)
+    refused(1, api.i8_norm_rows, x, 4, 32, None, 1e-5, c, s.half())
+    refused(1, api.i8_matmul, c.short(), s, 4, codes(8), torch.zeros(8), 8, 32, torch.zeros((4, 8)))
+    refused(1, api.i8_matmul, c, s.half(), 4, codes(8), torch.zeros(8), 8, 32, torch.zeros((4, 8)))
+    refused(1, api.i8_matmul, c, s, 4, codes(8).short(), torch.zeros(8), 8, 32, torch.zeros((4, 8)))
+    refused(1, api.i8_matmul, c, s, 4, codes(8), torch.zeros(8).double(), 8, 32, torch.zeros((4, 8)))
+    for n, kind in ((0, torch.float64), (1, torch.int64), (2, torch.int64), (3, torch.bfloat16)):
+        given = [torch.zeros((4, 4)), i, i.clone(), torch.zeros((4, 4))]
+        given[n] = given[n].to(kind)
+        refused(1, api.beam_select, torch.zeros((16, 10)), given[0], 4, 4, 10, 4, *given[1:])
+    refused(1, api.beam_reorder, x, x.clone(), i.long(), 1, 4, 4, 1, 1, 8)
+    refused(1, api.beam_reorder, x, x.clone(), i, 1, 4, 4, 1, 1, 8, d_lengths=i[0].long())
+
+
 def test_without_a_device_there_is_no_fallback():
     if api.device_count() > 0:
         pytest.skip("a GPU is present")
