@@ -126,10 +126,11 @@ __device__ __forceinline__ float warp_larger(float v) {
 }
 
 // Blocks of MOST threads that an SM's registers shall hold.
-// (16,384 x 8,192 bf16 with norm: 3 170 us, 4 164, 5 216; rows that begin anywhere, 200,000 x 500: 3 141, 4 160; 30,000 x 4,096 without: 4 68, 5 64.5, 6 63; fp32,
+// (16,384 x 8,192 bf16 with norm, at full clocks and after a second at the power limit: 3 170 us and 170 to 182, 4 164 and 175 to 186, 5 216; rows that begin
+// anywhere, 200,000 x 500: 3 141, 4 160; 30,000 x 4,096 without: 4 68, 5 64.5, 6 63; fp32,
 // 100,000 x 1,000 with norm: 4 189, 5 225; 1M x 96 without: 6 74, 7 70; 100,000 x 333: 6 34, 7 38; blocks of 512, 8,000 x 16,384 bf16 with norm: 1 235, 2 181, without 125 and 85)
 template <int kEach, int MOST, bool NORM, bool SHIFT> constexpr int blocks_of() {
-    return MOST == 256 ? (kEach == 32 ? (NORM ? (SHIFT ? 3 : 4) : 6) : NORM ? 4 : SHIFT ? 6 : 7) : MOST == 288 || (MOST == 512 && !(NORM && SHIFT)) ? 2 : 1;
+    return MOST == 256 ? (kEach == 32 ? (NORM ? 3 : 6) : NORM ? 4 : SHIFT ? 6 : 7) : MOST == 288 || (MOST == 512 && !(NORM && SHIFT)) ? 2 : 1;
 }
 
 // One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM, SHIFT>()))
     const float inverse = top32 > 0 ? 127.f / top32 : 0.f;
     signed char* out = a.codes + (live ? row : 0) * a.code_stride;
     float off = 0.f;   // the furthest from a whole number
-    const unsigned long long by = pair(inverse, inverse), whole = pair(kRint, kRint), back = pair(-kRint, -kRint), minus = pair(-1.f, -1.f);
+    const unsigned long long by = pair(inverse, inverse), whole = pair(kRint, kRint), back = pair(-kRint, -kRint), less = pair(-inverse, -inverse);
     unsigned c[kEach];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM, SHIFT>()))
             const int i = (j * VEC + e) / 2;
             unsigned long long u = h[i];
             if (NORM) u = mul2(u, pair(pw.get(e), pw.get(e + 1)));
-            const unsigned long long m = fma2(u, by, whole), away = fma2(u, by, mul2(add2(m, back), minus));
+            const unsigned long long m = fma2(u, by, whole), away = fma2(u, less, add2(m, back));
             const float2 code = halves(m), d = halves(away);
             c[2 * i] = __float_as_uint(code.x);
             c[2 * i + 1] = __float_as_uint(code.y);
