@@ -128,9 +128,9 @@ __device__ __forceinline__ float warp_larger(float v) {
 // Blocks of MOST threads that an SM's registers shall hold.
 // (16,384 x 8,192 bf16 with norm, at full clocks and after a second at the power limit: 3 170 us and 170 to 182, 4 164 and 175 to 186, 5 216; rows that begin
 // anywhere, 200,000 x 500: 3 141, 4 160; 30,000 x 4,096 without: 4 68, 5 64.5, 6 63; fp32,
-// 100,000 x 1,000 with norm: 4 189, 5 225; 1M x 96 without: 6 74, 7 70; 100,000 x 333: 6 34, 7 38; blocks of 512, 8,000 x 16,384 bf16 with norm: 1 235, 2 181, without 125 and 85)
+// 100,000 x 1,000 with norm: 4 189, 5 225; 1M x 96 without, 16 elements a thread: 6 74, 7 70; 100,000 x 333: 6 34, 7 38; blocks of 512, 8,000 x 16,384 bf16 with norm: 1 235, 2 181, without 125 and 85)
 template <int kEach, int MOST, bool NORM, bool SHIFT> constexpr int blocks_of() {
-    return MOST == 256 ? (kEach == 32 ? (NORM ? 3 : 6) : NORM ? 4 : SHIFT ? 6 : 7) : MOST == 288 || (MOST == 512 && !(NORM && SHIFT)) ? 2 : 1;
+    return MOST == 256 ? (kEach >= 24 ? (NORM ? 3 : 6) : NORM ? 4 : SHIFT ? 6 : 7) : MOST == 288 || (MOST == 512 && !(NORM && SHIFT)) ? 2 : 1;
 }
 
 // One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in
@@ -550,6 +550,16 @@ psb_status start(const RowArgs& a, int threads, int sms, cudaStream_t s) {
     return PSB_OK;
 }
 
+// TPR threads a row, each with three quarters of the elements where those hold it (at the power limit: 1M x 96 fp32 82.4 us, so 79.2; 500,000 x 96 bf16 with norm 72.7 and 66.8;
+// 60,000 x 768 68.8 and 63.8).
+template <typename T, int TPR, bool NORM, bool SHIFT>
+psb_status start_of(const RowArgs& a, int sms, cudaStream_t s) {
+    constexpr int kMost = Pack<T>::VEC == 8 ? 32 : 16;
+    if constexpr (!SHIFT)
+        if (a.dim <= TPR * kMost / 4 * 3) return start<T, kMost / 4 * 3, TPR, 256, NORM, SHIFT>(a, 0, sms, s);
+    return start<T, kMost, TPR, 256, NORM, SHIFT>(a, 0, sms, s);
+}
+
 // As few threads a row as hold it in registers, 32 elements of two bytes or 16 of four each, since what a thread does once a row is then shared among
 // most (16,384 rows of 8,192 in bf16: 172 us with 32 elements, 212 with 16); more of them, with 16 elements, where rows are too few to fill the
 // GPU (one row of 4,096: 3.0 us, with 32 3.6).
@@ -563,11 +573,12 @@ psb_status by_length(const RowArgs& a, int sms, cudaStream_t s) {
         while (threads <= 512 && threads < warps(VEC) && a.n * (long long)threads * 2 <= 1024ll * sms) threads *= 2;   // (all rows at once)
         return start<T, 16, 0, 1024, NORM, SHIFT>(a, std::min(threads, warps(VEC)), sms, s);
     }
-    if (span <= 4 * 16) return start<T, 16, 4, 256, NORM, SHIFT>(a, 0, sms, s);
-    if (span <= 4 * kMost) return start<T, kMost, 4, 256, NORM, SHIFT>(a, 0, sms, s);
-    if (span <= 8 * kMost) return start<T, kMost, 8, 256, NORM, SHIFT>(a, 0, sms, s);
-    if (span <= 16 * kMost) return start<T, kMost, 16, 256, NORM, SHIFT>(a, 0, sms, s);
-    if (span <= 32 * kMost) return start<T, kMost, 32, 256, NORM, SHIFT>(a, 0, sms, s);
+    if constexpr (VEC == 8)
+        if (span <= 4 * 16) return start<T, 16, 4, 256, NORM, SHIFT>(a, 0, sms, s);
+    if (span <= 4 * kMost) return start_of<T, 4, NORM, SHIFT>(a, sms, s);
+    if (span <= 8 * kMost) return start_of<T, 8, NORM, SHIFT>(a, sms, s);
+    if (span <= 16 * kMost) return start_of<T, 16, NORM, SHIFT>(a, sms, s);
+    if (span <= 32 * kMost) return start_of<T, 32, NORM, SHIFT>(a, sms, s);
     if (span <= 256 * kMost) return start<T, kMost, 0, 256, NORM, SHIFT>(a, warps(kMost), sms, s);
     if (span <= 288 * kMost) return start<T, kMost, 0, 288, NORM, SHIFT>(a, warps(kMost), sms, s);
     if (span <= 512 * kMost) return start<T, kMost, 0, 512, NORM, SHIFT>(a, warps(kMost), sms, s);

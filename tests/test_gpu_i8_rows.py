@@ -89,6 +89,13 @@ def test_many_rows(psb, t, n, dim):
     check_scales(scales, scale)
 
 
+# both sides of the lengths to which a thread of a warp has three quarters of its elements, and few rows of them
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n,dim", [(40000, 48), (40001, 52), (20000, 72), (30000, 96), (3, 96), (30001, 104), (20000, 192), (20001, 200), (10000, 384), (1, 384), (9000, 392), (6000, 768), (6001, 776)])
+def test_three_quarters(psb, t, n, dim):
+    test_many_rows(psb, t, n, dim)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("dim,pads", [(96, (3, 5, 7, 9)), (96, (8, 16, 24, 32)), (1000, (0, 1, 0, 0)), (4096, (8, 8, 8, 16)), (50, (1, 1, 1, 1))])
 @pytest.mark.parametrize("where", ["apart", "rows", "residual"])
