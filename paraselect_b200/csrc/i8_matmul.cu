@@ -105,18 +105,35 @@ __device__ __forceinline__ Scales scales_of(const MatmulArgs& a, bool there, int
     return Scales{there && c < a.n ? __ldg(a.w_scales + c) : 0.f, there && token < a.tokens && t0 + token < a.m ? __ldg(a.x_scales + t0 + token) : 0.f};
 }
 
+// The end of a wait, for all lanes of a warp alike: where one gave up, all did.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int polls) { return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, polls)); }
+
+// A named barrier of whole warps; true where every thread says so.
+__device__ __forceinline__ bool all_of(bool ok, int barrier, int threads) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.and.pred p, %2, %3, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)ok), "r"(barrier), "r"(threads)
+        : "memory");
+    return r != 0;
+}
+
 // An epilogue warp's columns of a tile, 32 channels: channel c in this thread, tokens from t0.  SOLO: the four warps of this half of the epilogue have the tile
-// to themselves (its tokens are 32 at most), otherwise each half takes every other 16 tokens; all warps that share the tile call it.
+// to themselves (its tokens are 32 at most), otherwise each half takes every other 16 tokens; all warps that share the tile call it, whether their wait
+// for it ended well (`ready`) or not: where one's did not, none stores and all leave, so that no warp is waited for that has left.
 // `scales`: the other of the two buffers still serves slower warps' last tile.
 template <typename T, bool SOLO>
-__device__ __forceinline__ void store_tile(const MatmulArgs& a, float* scales, const Scales& own, uint32_t from, int c, int t0, int warp, int lane) {
+__device__ __forceinline__ bool store_tile(const MatmulArgs& a, bool ready, float* scales, const Scales& own, uint32_t from, int c, int t0, int warp, int lane) {
     const int half = SOLO ? 0 : warp >> 2, every = SOLO ? 16 : 32;
     if (SOLO) scales += warp >> 2 << 7;
     scales[(SOLO ? warp & 3 : warp) * 32 + lane] = own.x;
     const bool here = c < a.n;
     const float ws = own.w;
-    if (SOLO) asm volatile("bar.sync %0, %1;" ::"r"(1 + (warp >> 2)), "n"(16 * kEpilogue) : "memory");
-    else asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogue) : "memory");
+    if (!all_of(ready, SOLO ? 1 + (warp >> 2) : 1, SOLO ? 16 * kEpilogue : 32 * kEpilogue)) return false;
     T* out = static_cast<T*>(a.out) + (long long)(t0 + half * 16) * a.out_stride + c;
     const int live = min(a.tokens, a.m - t0);
     for (int t = half * 16; t < live; t += every, out += every * a.out_stride) {
@@ -138,6 +155,7 @@ __device__ __forceinline__ void store_tile(const MatmulArgs& a, float* scales, c
             }
         }
     }
+    return true;
 }
 
 // Where a block gave up, the copies that are under way to its ring land before it ends.  For one thread.
@@ -248,13 +266,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
             const int c0 = tile % a.channel_tiles * kChannels, t0 = tile / a.channel_tiles * a.tokens;
             const Scales own = next;
             next = scales(tile + turns * step);
-            if (!tc::mbar_wait(&ready[buf], (count / kBuffers) & 1, a.polls)) { gave_up = 1; break; }
-            __syncwarp();
+            const bool ok = warp_wait(&ready[buf], (count / kBuffers) & 1, a.polls);
             tc::tc_fence_after();
             const int quarter = warp & 3, half = warp >> 2;
             const uint32_t from = tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16);
             const int c = quarter * 32 + lane;
             if constexpr (SPLIT) {   // all products have ended: the ring is free for the partial sums, [token][channel]
+                if (!ok) { gave_up = 1; break; }
                 int* partial = reinterpret_cast<int*>(ring);
                 for (int t = half * 16; t < a.tokens; t += 32) {
                     uint32_t v[16];
@@ -264,8 +282,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
                     for (int i = 0; i < 16; ++i) partial[(t + i) * kChannels + c] = (int)v[i];
                 }
             } else {
-                if (solo) store_tile<T, true>(a, s_scales[count / 2 & 1], own, from, c0 + c, t0, warp, lane);
-                else store_tile<T, false>(a, s_scales[count & 1], own, from, c0 + c, t0, warp, lane);
+                const bool stored = solo ? store_tile<T, true>(a, ok, s_scales[count / 2 & 1], own, from, c0 + c, t0, warp, lane)
+                                         : store_tile<T, false>(a, ok, s_scales[count & 1], own, from, c0 + c, t0, warp, lane);
+                if (!stored) { gave_up = 1; break; }
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&drained[buf])) : "memory");
@@ -453,11 +472,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
             place_of(a, tile, &c0, &t0);
             const Scales own = next;
             next = scales(tile + step);
-            if (!tc::mbar_wait(&ready[buf], (count / 2) & 1, a.polls)) { gave_up = 1; break; }
-            __syncwarp();
+            const bool ok = warp_wait(&ready[buf], (count / 2) & 1, a.polls);
             tc::tc_fence_after();
             const int quarter = warp & 3;
-            store_tile<T, false>(a, s_scales[count & 1], own, tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16), c0 + rank * kChannels + quarter * 32 + lane, t0, warp, lane);
+            if (!store_tile<T, false>(a, ok, s_scales[count & 1], own, tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16), c0 + rank * kChannels + quarter * 32 + lane, t0, warp,
+                                      lane)) {
+                gave_up = 1;
+                break;
+            }
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(&drained[buf])) : "memory");

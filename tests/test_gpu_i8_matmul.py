@@ -152,3 +152,13 @@ def test_many_streams_of_split_paired_and_single_products(psb):
     torch.cuda.synchronize()
     for s, x, xs, w, ws, out, m, n, k in calls:
         assert close(out, expected(x, xs, w, ws, k), torch.float32)
+
+
+# Single blocks that run through several tiles, the tile's tokens for one half of the epilogue (20, 32) and for both (33, 100, 250), and pairs with tiles left over: the
+# warps that share a tile have to agree on how their wait ended.
+@pytest.mark.parametrize("m,n,k,tiles", [(20, 40000, 128, 0), (20, 40000, 128, 100), (20, 40000, 128, 200), (20, 40000, 128, 312), (32, 30000, 700, 170), (33, 40000, 100, 150),
+                                         (100, 40000, 128, 0), (100, 40000, 128, 100), (100, 40000, 128, 200), (100, 30011, 700, 149), (180, 20000, 260, 155),
+                                         (2000, 4000, 128, 60), (2000, 4000, 1100, 80), (250, 40001, 300, 100)])
+def test_results_when_a_wait_of_single_blocks_or_pairs_gives_up(psb, m, n, k, tiles):
+    for t in TYPES:
+        check(psb, m, n, k, t, limited=tiles)
