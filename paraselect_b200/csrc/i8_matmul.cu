@@ -10,8 +10,8 @@
 // rows behind the last are the TMA's zeros.  Few tiles are split along k over a cluster of up to 8 blocks, which hold their partial sums in
 // shared memory and add them there: integers, so the order does not matter.
 //
-// Waits on the device are bounded.  A block whose wait gave up waits for what it has issued, frees its tensor memory and forms its outputs
-// with dp4a instead, so that the results are the same.
+// Waits on the device are bounded.  A block one of whose waits gave up, whichever role's, waits for the products and copies that it has issued, frees
+// its tensor memory and forms its outputs with dp4a instead, so that the results are the same.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -158,9 +158,9 @@ __device__ __forceinline__ bool store_tile(const MatmulArgs& a, bool ready, floa
     return true;
 }
 
-// Where a block gave up, the copies that are under way to its ring land before it ends.  For one thread.
-__device__ __forceinline__ void await_loads(uint64_t* full, int loads, int stages, int polls) {
-    for (int i = max(0, loads - stages); i < loads; ++i) tc::mbar_wait(&full[i % stages], (i / stages) & 1, polls);
+// Where a block gave up, the copies that are under way to its ring land before it ends.  For one thread.  (They land whatever the call's own limit is.)
+__device__ __forceinline__ void await_loads(uint64_t* full, int loads, int stages) {
+    for (int i = max(0, loads - stages); i < loads; ++i) tc::mbar_wait(&full[i % stages], (i / stages) & 1);
 }
 
 // SPLIT: the blocks of a cluster share a tile, each with its share of the slabs.  Otherwise a block takes every gridDim.x-th tile, its
@@ -245,11 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
                 }
                 if (ok) tc::umma_commit(&ready[buf]);
             }
-            if (!ok) {   // the products under way end before the tensor memory is freed
-                gave_up = 1;
-                tc::umma_commit(&last);
-                tc::mbar_wait(&last, 0, a.polls);
-            }
+            if (!ok) gave_up = 1;
         }
         __syncwarp();
     } else {
@@ -294,8 +290,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul(const __grid_constant
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
+    if (gave_up) {   // whichever role did: the products and copies under way end before the tensor memory is freed and the ring left
+        if (warp == kEpilogue + 1) {
+            if (tc::elect_one()) {   // the thread that issued them
+                tc::umma_commit(&last);
+                tc::mbar_wait(&last, 0);
+            }
+            __syncwarp();
+        }
+        if (threadIdx.x == 0) await_loads(full, loads, a.stages);
+        tc::tc_fence_before();
+        __syncthreads();
+        tc::tc_fence_after();
+    }
     if (warp == kEpilogue + 1) tc::tmem_dealloc(tmem, tmem_columns(a.tokens, kBuffers));
-    if (gave_up && threadIdx.x == 0) await_loads(full, loads, a.stages, a.polls);
 
     if constexpr (SPLIT) {
         cg::cluster_group cluster = cg::this_cluster();
@@ -451,11 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
                 }
                 if (ok) pair_commit(&ready[buf]);
             }
-            if (!ok) {   // the products under way end before the tensor memory is freed
-                gave_up = 1;
-                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc::smem_u32(&last)) : "memory");
-                tc::mbar_wait(&last, 0, a.polls);
-            }
+            if (!ok) gave_up = 1;
         }
         __syncwarp();
     } else {
@@ -488,9 +492,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
     tc::tc_fence_before();
     cluster.sync();
     tc::tc_fence_after();
-    if (warp == kEpilogue + 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
     const int lost = gave_up | *cluster.map_shared_rank(&gave_up, rank ^ 1);
-    if (lost && rank == 0 && threadIdx.x == 0) await_loads(full, loads, a.stages, a.polls);   // (both blocks' copies count here)
+    if (lost) {   // whichever block and role gave up: the products and copies under way end before the tensor memory is freed and the rings left
+        if (warp == kEpilogue + 1) {
+            if (tc::elect_one()) {   // in the first block the thread that issued them; both blocks' barriers hear of their end
+                if (rank == 0) pair_commit(&last);
+                tc::mbar_wait(&last, 0);
+            }
+            __syncwarp();
+        }
+        if (rank == 0 && threadIdx.x == 0) await_loads(full, loads, a.stages);   // (both blocks' copies count here)
+        tc::tc_fence_before();
+        cluster.sync();
+        tc::tc_fence_after();
+    }
+    if (warp == kEpilogue + 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
     cluster.sync();   // neither block ends while the other looks
     if (lost) {
         for (int tile = first; tile < a.tiles; tile += step) {
