@@ -388,6 +388,16 @@ __device__ __forceinline__ void place_of(const MatmulArgs& a, int tile, int* c0,
     *t0 = (first + i % beside) * a.tokens;
 }
 
+// Where a pair gave up: the copies of both blocks land, which count on the first block's barriers.  The blocks need not have come equally far.  A stage that one of them
+// alone has filled expects both blocks' bytes if it is the first block (`mine` > `other`): the second's are made up for; if it is the second, nobody has told the
+// barrier to expect anything.  No more such stages than the ring has, since their last filling before has been consumed.  For one thread of the first block.
+__device__ __forceinline__ void await_pair_loads(uint64_t* full, int mine, int other, int stages, int stage_bytes) {
+    for (int i = other; i < mine; ++i)
+        asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(tc::smem_u32(&full[i % stages])), "r"(stage_bytes) : "memory");
+    for (int i = mine; i < other; ++i) tc::mbar_expect_tx(&full[i % stages], stage_bytes);
+    await_loads(full, max(mine, other), stages);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MatmulArgs a) {
     extern __shared__ unsigned char raw[];
@@ -501,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
             }
             __syncwarp();
         }
-        if (rank == 0 && threadIdx.x == 0) await_loads(full, loads, a.stages);   // (both blocks' copies count here)
+        if (rank == 0 && threadIdx.x == 0) await_pair_loads(full, loads, *cluster.map_shared_rank(&loads, 1), a.stages, stage_bytes);
         tc::tc_fence_before();
         cluster.sync();
         tc::tc_fence_after();

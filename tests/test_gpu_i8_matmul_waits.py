@@ -9,7 +9,7 @@ import torch
 from test_gpu_i8_matmul import close, codes, expected, scales
 
 pytestmark = pytest.mark.gpu
-POLLS = [1, 2, 5, 20, 100]
+POLLS = [1, 2, 3, 5, 8, 12, 20, 100]
 
 
 def check(psb, m, n, k, polls):
@@ -27,4 +27,11 @@ def check(psb, m, n, k, polls):
 @pytest.mark.parametrize("polls", POLLS)
 @pytest.mark.parametrize("m,n,k", [(20, 18000, 1000), (20, 37000, 128), (20, 50000, 300), (100, 18000, 4000), (100, 37000, 128), (180, 50000, 260), (40, 700, 4096), (130, 130, 9000)])
 def test_single_and_split(psb, m, n, k, polls):
+    check(psb, m, n, k, polls)
+
+
+# pairs of blocks, whose two loading threads give up by themselves, so that one may have come further than the other
+@pytest.mark.parametrize("polls", POLLS)
+@pytest.mark.parametrize("m,n,k", [(200, 18000, 2000), (250, 30001, 300), (256, 18000, 128), (1000, 9000, 1100), (2000, 4000, 4096), (3000, 2561, 300)])
+def test_pairs(psb, m, n, k, polls):
     check(psb, m, n, k, polls)
