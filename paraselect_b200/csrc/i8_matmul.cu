@@ -443,6 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_i8_matmul_pair(const __grid_con
                     pair_load(to + kChannels * kSlab, &map_x, slab * kSlab, t0 + rank * mine, in_first(&full[st]));
                 }
             }
+            // the other block's thread releases the ring's last stages here too: this block does not end before
+            for (int i = max(0, at - a.stages); ok && i < at; ++i) ok = tc::mbar_wait(&empty[i % a.stages], (i / a.stages) & 1, a.polls);
             loads = at;
             if (!ok) gave_up = 1;
         }
