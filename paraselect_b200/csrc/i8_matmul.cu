@@ -714,10 +714,13 @@ psb_status codes_map(CUtensorMap* map, const void* base, int64_t rows, int k, in
     return PSB_OK;
 }
 
+// The tokens of each of `tiles` tiles of even size, a multiple of `step`.  (m + tiles leaves 32 bits from 2,139,127,681 rows on.)
+int tokens_of(int m, int tiles, int step) { return (int)(((long long)m + tiles - 1) / tiles + step - 1) / step * step; }
+
 template <typename T>
 psb_status run_pairs(MatmulArgs a, int sms, cudaStream_t s) {
     const int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
-    a.tokens = ((a.m + token_tiles - 1) / token_tiles + 31) / 32 * 32;
+    a.tokens = tokens_of(a.m, token_tiles, 32);
     a.channel_tiles = (a.n + 2 * kChannels - 1) / (2 * kChannels);
     const long long tiles = (long long)token_tiles * a.channel_tiles;
     if (tiles > 0x3fffffff) return fail(PSB_UNSUPPORTED_SHAPE, "product of codes: more than 2^30 - 1 tiles of 256 x 256 outputs");
@@ -753,7 +756,7 @@ psb_status run(MatmulArgs a, int sms, cudaStream_t s) {
     a.channel_tiles = (a.n + kChannels - 1) / kChannels;
     int token_tiles = (a.m + kMaxTokens - 1) / kMaxTokens;
     if (token_tiles > 1 && (long long)token_tiles * a.channel_tiles * 2 < sms) token_tiles = (a.m + 127) / 128;
-    a.tokens = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    a.tokens = tokens_of(a.m, token_tiles, 16);
     const long long tiles = (long long)token_tiles * a.channel_tiles;
     // Pairs and single blocks: 1,024 x 32,000 x 4,096 96.9 and 122.8 us, 256 x 14,336 x 4,096 19.5 and 20.9, 200 x 32,000 x 4,096 32.1 and 33.6, 1,024 x 4,096 x 4,096 17.9 and 18.5
     if (a.m >= kPairMin && tiles * 2 >= sms) return run_pairs<T>(a, sms, s);

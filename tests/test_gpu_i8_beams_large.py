@@ -82,3 +82,23 @@ def test_states(psb, place):
     want = torch.tensor([4, 1, 1, 3], device="cuda", dtype=torch.bfloat16)
     assert torch.equal(out[-1, -1, :, -1, -1, 0], want) and torch.equal(out[0, 0, :, 0, 0, -1], want + 10)
     assert out[:, :, :, :, 1:-1].count_nonzero() == 0
+
+
+@pytest.mark.parametrize("m,n", [((1 << 31) - 256, 1), (5, (1 << 31) - 256), (1, (1 << 31) - 256)])
+def test_products_of_the_most_rows(psb, m, n):
+    k = 16                                        # 34 GB of codes
+    g = torch.Generator(device="cuda").manual_seed(4)
+
+    def codes(rows):                              # zeros, but for rows at both ends and beside 2^30
+        c = torch.zeros((rows, k), dtype=torch.int8, device="cuda")
+        some = sorted({r for r in (0, 1, 200, 255, 256, 1 << 30, rows - 257, rows - 256, rows - 2, rows - 1) if 0 <= r < rows})
+        c[some] = torch.randint(-127, 128, (len(some), k), generator=g, device="cuda", dtype=torch.int8)
+        return c, some
+    x, xr = codes(m)
+    w, wr = codes(n)
+    xs, ws = torch.full((m,), 0.5, device="cuda"), torch.full((n,), 0.25, device="cuda")
+    out = torch.full((m, n), 7.0, dtype=torch.float16, device="cuda")
+    psb.i8_matmul(x, xs, m, w, ws, n, k, out)
+    want = (x[xr].double() @ w[wr].double().T) * 0.125     # halves of eighths: at most 17 bits
+    assert torch.equal(out[xr][:, wr], want.half())
+    assert int(out.count_nonzero()) == int(want.count_nonzero())   # and zeros everywhere else
