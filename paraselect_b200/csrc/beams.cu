@@ -5,9 +5,12 @@
 // lowest (beam, token).  One cluster of blocks takes an item, and the logits are read once: a warp reduces its share of a beam's row to a
 // maximum and a sum, and to the maxima of groups of its lanes.  From those every block has each beam's log-sum, and a bound that k of the
 // groups' maxima, as totals, reach, so that at least k totals do.  Only the parts of a share whose maximum reaches the bound are looked through
-// again; the few totals found are ranked by the cluster's first block.  Sums are held in fp32 within a lane (some hundred terms) and in 64 bits
-// beyond, totals are compared in 64 bits.  The warps of a cluster are dealt out to the beams, so that a warp of a small call waits for one
-// round of loads and reduces once.
+// again; the few totals found are ranked by the cluster's first block.  The warps of a cluster are dealt out to the beams, so that a warp of a small
+// call waits for one round of loads and reduces once.
+//
+// A lane adds its exponentials in fp32: a step's (16 or 32) in chains of four, the steps' sums with compensation, so that the error does not grow with the
+// vocabulary (added one after the other, a lane's terms, where they are alike, were 2e-5 off with 100,000 tokens and 9e-4 with 4 million).  Beyond a lane sums are held in
+// 64 bits, and totals are compared in 64 bits.
 //
 // What a lane reads and adds depends on the tokens' numbers alone, not on a row's address, so that equal rows have equal totals.
 #include <cooperative_groups.h>
@@ -194,14 +197,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
     SelectShared& s = *reinterpret_cast<SelectShared*>(raw);
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const long long item = blockIdx.x / blocks;
+    const int item = (int)blockIdx.x / blocks;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int warps = blocks * kWarps, me = rank * kWarps + warp, shares = a.per_beam * a.beams;
-    const T* rows = static_cast<const T*>(a.logits) + item * a.beams * a.row_stride;
     auto beam_of = [&](int share) { return a.per_beam == 1 ? share : (int)__umulhi((unsigned)share, a.by_beam); };   // exact: shares are below 2^16
     auto part_of = [&](int share) { return share - beam_of(share) * a.per_beam; };
+    auto row_of = [&](int share) { return static_cast<const T*>(a.logits) + ((long long)item * a.beams + beam_of(share)) * a.row_stride; };
     if (threadIdx.x == 0) s.count = 0;
-    if (threadIdx.x < a.beams) s.score[threadIdx.x] = a.scores[item * a.beams + threadIdx.x];
+    if (threadIdx.x < a.beams) s.score[threadIdx.x] = a.scores[(long long)item * a.beams + threadIdx.x];
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // waited for before the first write to another block
 
     // A share's lines are per_beam apart, kLines of them at a time, read ahead by as many.
@@ -217,15 +220,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
         }
     };
     for (int share = me, turn = 0; share < shares; share += warps, ++turn) {
-        const T* row = rows + beam_of(share) * a.row_stride;
+        const T* row = row_of(share);
         float top = -INFINITY, at = 0.f, part = -INFINITY;
         float best = -INFINITY, second = -INFINITY, third = -INFINITY;   // of this lane's steps
         unsigned which = 0;                                             // best's number in the low half, second's in the high
-        unsigned long long sums = 0;   // two sums of zero
+        unsigned long long sums = 0, rest = 0;   // two sums of zero, and what their roundings have left out
         Raw8<T> x[kLines], next[kLines];
         int line = part_of(share);
         read(row, line, x);
-#pragma unroll 2
+#pragma unroll 1   // (twice, registers spill: one item of 4 x 32,000 fp32 9.5 us instead of 8.9, 64 x 8 x 128,000 bf16 40.8 instead of 40.1)
         for (int step = 0; step < steps; ++step, line += kLines * a.per_beam) {
             if (step + 1 < steps) read(row, line + kLines * a.per_beam, next);
             unsigned m = Raw8<T>::kNone;
@@ -243,10 +246,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
             if (most > top) {   // the same for all lanes: the sums come down to the new base
                 const float to = most * kLog2e;
                 const float by = top == -INFINITY ? 0.f : huge(top) || huge(most) ? exp2_of((top - most) * kLog2e) : exp2_of(at - to);
-                const float2 v = halves(sums);
-                sums = pair(v.x * by, v.y * by);
+                sums = mul2(sums, pair(by, by));
+                rest = mul2(rest, pair(by, by));
                 top = most; at = to;
             }
+            unsigned long long more = 0;   // of this step
             if (huge(top) && top != -INFINITY) {
 #pragma unroll 1
                 for (int u = 0; u < kLines; ++u)
@@ -254,24 +258,35 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
                         Raw8<T> y;
                         y.read(row, (line + u * a.per_beam) * kLine + lane * 8, a.vocab, a.wide);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) { const float2 v = y.two(i); sums = add2(sums, pair(exp2_of((v.x - top) * kLog2e), exp2_of((v.y - top) * kLog2e))); }
+                        for (int i = 0; i < 4; ++i) { const float2 v = y.two(i); more = add2(more, pair(exp2_of((v.x - top) * kLog2e), exp2_of((v.y - top) * kLog2e))); }
                     }
             } else {
                 const unsigned long long scale = pair(kLog2e, kLog2e), less = pair(-at, -at);
+                unsigned long long of[kLines];
 #pragma unroll
                 for (int u = 0; u < kLines; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float2 v = x[u].two(i), e = halves(fma2(pair(v.x, v.y), scale, less));
-                        sums = add2(sums, pair(exp2_of(e.x), exp2_of(e.y)));
+                        const unsigned long long term = pair(exp2_of(e.x), exp2_of(e.y));
+                        of[u] = i ? add2(of[u], term) : term;
                     }
+#pragma unroll
+                for (int apart = kLines / 2; apart > 0; apart /= 2)
+#pragma unroll
+                    for (int u = 0; u < apart; ++u) of[u] = add2(of[u], of[u + apart]);
+                more = of[0];
             }
+            more = add2(more, rest);
+            const unsigned long long now = add2(sums, more), minus = pair(-1.f, -1.f);
+            rest = fma2(fma2(sums, minus, now), minus, more);   // more - (now - sums)
+            sums = now;
 #pragma unroll
             for (int u = 0; u < kLines; ++u) x[u] = next[u];
         }
         // without a finite maximum the sum is zero or, with a NaN or an infinity among the logits, NaN
-        const float2 v = halves(sums);
-        double sum = (double)v.x + (double)v.y;
+        const float2 v = halves(sums), r = halves(rest);
+        double sum = ((double)v.x + (double)r.x) + ((double)v.y + (double)r.y);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         s.parts[turn][warp][lane] = part;
@@ -358,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
         }
     };
     auto each = [&](int share, int turn, float least, auto&& what) {   // of a share's tokens those of the parts that reach `least`
-        const T* row = rows + beam_of(share) * a.row_stride;
+        const T* row = row_of(share);
         const unsigned parts = __ballot_sync(0xffffffffu, s.parts[turn][warp][lane] >= least);
 #pragma unroll 1
         for (int step = 0; step < steps; ++step)
@@ -379,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
         const float4 top = s.steps[turn][warp][lane];
         if (__any_sync(0xffffffffu, top.z >= least)) { each(share, turn, least, take); continue; }
         // no lane has more than two steps that reach it: every lane reads its own, all at once
-        const T* row = rows + b * a.row_stride;
+        const T* row = row_of(share);
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             const bool there = (i ? top.y : top.x) >= least;
@@ -450,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
         int place = 0;
         for (int o = 0; o < n; ++o) place += before(s.found[o], mine);
         if (place < a.k) {
-            const long long to = item * a.k + place;
+            const long long to = (long long)item * a.k + place;
             const unsigned parent = mine.at / (unsigned)a.vocab;
             a.parents[to] = (int)parent;
             a.tokens[to] = (int)(mine.at - parent * (unsigned)a.vocab);
@@ -458,9 +473,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
         }
     }
     for (int i = n + threadIdx.x; i < a.k; i += kThreads) {
-        a.parents[item * a.k + i] = -1;
-        a.tokens[item * a.k + i] = -1;
-        a.totals[item * a.k + i] = -INFINITY;
+        const long long to = (long long)item * a.k + i;
+        a.parents[to] = -1;
+        a.tokens[to] = -1;
+        a.totals[to] = -INFINITY;
     }
 }
 
