@@ -130,13 +130,14 @@ __device__ __forceinline__ double from_ordered(unsigned long long o) { return __
 struct Found { unsigned long long total; unsigned at; unsigned pad; };   // at = beam * vocab + token
 __device__ __forceinline__ bool before(const Found& a, const Found& b) { return a.total > b.total || (a.total == b.total && a.at < b.at); }
 
-// The largest logit, and the sum of exp2((x - base) kLog2e) over the share's tokens.  base = (top kLog2e) (1 / kLog2e) with the product rounded to fp32,
-// so that an exponent takes one fused operation and what the rounding changed is known; where that product leaves fp32, the logit itself.
-struct Share { float top; double sum; };
-__device__ __forceinline__ bool huge(float top) { return fabsf(top) > 1e38f; }
-__device__ __forceinline__ double base_of(float top) { return huge(top) ? (double)top : (double)(top * kLog2e) * (1.0 / (double)kLog2e); }
+// The largest logit, and the sum of exp2((x - base) kLog2e) over the share's tokens.  base kLog2e is a whole number, `at`, the next above the largest logit's (or kLow,
+// below every logit within kFar): an exponent is one fused operation, x kLog2e - at, exact but for its own rounding, and where a larger logit comes, the sum goes
+// down by a power of two, exactly.  Where the largest logit lies beyond kFar, `at` cannot hold its fraction (from 1e10 on its own exponent came out in the
+// hundreds, and its beam's sum as zero or infinite): such a share is summed again, less the largest logit, which is then the base.
+struct Share { float top, at; double sum; };   // at: as long as |top| <= kFar
+constexpr float kFar = 4e6f, kLow = -5770781.f;
 
-// 2^v for v <= 0 with a relative error below 1e-9: the Taylor series of e^(f ln 2), |f| <= 1/2, to the eighth power.  (CUDA's own, exact to the last of
+// 2^v for v <= 2 with a relative error below 1e-9: the Taylor series of e^(f ln 2), |f| <= 1/2, to the eighth power.  (CUDA's own, exact to the last of
 // 53 bits, took a quarter of a small call's time.)
 __device__ __forceinline__ double exp2_64(double v) {
     if (!(v > -1000.0)) return v == v ? 0.0 : v;
@@ -146,7 +147,7 @@ __device__ __forceinline__ double exp2_64(double v) {
     p = fma(p, f, 1.0 / 6); p = fma(p, f, 0.5); p = fma(p, f, 1.0); p = fma(p, f, 1.0);
     return p * __longlong_as_double((long long)((int)n + 1023) << 52);
 }
-// log v for 1/2 <= v <= 2^25, in fp32 and one step of Newton's method on e^y = v, whose error is the square of fp32's.
+// log v for 1/4 <= v <= 2^25, in fp32 and one step of Newton's method on e^y = v, whose error is the square of fp32's.
 __device__ __forceinline__ double log_64(double v) {
     const double y = (double)logf((float)v), e = v * exp2_64(-y * 1.4426950408889634) - 1.0;
     return y + (e - 0.5 * e * e);
@@ -166,6 +167,21 @@ struct SelectShared {
     Found all[kMaxCluster][kMaxChosen];              // in the cluster's first block: what every block found
     int counts[kMaxCluster], first[kMaxCluster + 1];
 };
+
+// A lane's part of a share's sum of exp2((x - top) kLog2e), for logits too far from zero for the loop that takes all others.  (Not part of the kernel's code, whose
+// registers it would take.)
+template <typename T>
+__device__ __noinline__ double far_sum(const T* row, int line, int lines, int apart, int vocab, bool wide, float top) {
+    double sum = 0;
+#pragma unroll 1
+    for (; line < lines; line += apart) {
+        Raw8<T> x;
+        x.read(row, line * kLine + (int)(threadIdx.x & 31) * 8, vocab, wide);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const float2 v = x.two(i); sum += (double)exp2_of((v.x - top) * kLog2e) + (double)exp2_of((v.y - top) * kLog2e); }
+    }
+    return sum;
+}
 
 // The found ones beyond the k best go; the k best stay in no order.  For all threads of the block.
 __device__ void keep_best(SelectShared& s, int k) {
@@ -221,14 +237,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
     };
     for (int share = me, turn = 0; share < shares; share += warps, ++turn) {
         const T* row = row_of(share);
-        float top = -INFINITY, at = 0.f, part = -INFINITY;
+        float at = kLow, part = -INFINITY;
         float best = -INFINITY, second = -INFINITY, third = -INFINITY;   // of this lane's steps
         unsigned which = 0;                                             // best's number in the low half, second's in the high
         unsigned long long sums = 0, rest = 0;   // two sums of zero, and what their roundings have left out
         Raw8<T> x[kLines], next[kLines];
         int line = part_of(share);
         read(row, line, x);
-#pragma unroll 1   // (twice, registers spill: one item of 4 x 32,000 fp32 9.5 us instead of 8.9, 64 x 8 x 128,000 bf16 40.8 instead of 40.1)
+#pragma unroll 1   // (twice, registers spill: 64 x 8 x 128,000 bf16 42.1 us instead of 40.0)
         for (int step = 0; step < steps; ++step, line += kLines * a.per_beam) {
             if (step + 1 < steps) read(row, line + kLines * a.per_beam, next);
             unsigned m = Raw8<T>::kNone;
@@ -238,62 +254,49 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
                 for (int i = 0; i < Raw8<T>::kWords; ++i) m = Raw8<T>::larger(m, x[u].word[i]);
             const float t = Raw8<T>::largest(m);
             const float most = warp_max(t);
+            if (const float to = ceilf(most * kLog2e); to > at) {   // the same for all lanes: the sums come down to the new base
+                const float by = at - to >= -126.f ? __int_as_float(((int)(at - to) + 127) << 23) : 0.f;
+                sums = mul2(sums, pair(by, by));
+                rest = mul2(rest, pair(by, by));
+                at = to;
+            }
             which = t > best ? which << 16 | (unsigned)step : t > second ? (which & 0xffffu) | (unsigned)step << 16 : which;
             third = t > second ? second : fmaxf(third, t);
             second = t > best ? best : fmaxf(second, t);
             best = fmaxf(best, t);
             if (lane == step >> shift) part = fmaxf(part, most);
-            if (most > top) {   // the same for all lanes: the sums come down to the new base
-                const float to = most * kLog2e;
-                const float by = top == -INFINITY ? 0.f : huge(top) || huge(most) ? exp2_of((top - most) * kLog2e) : exp2_of(at - to);
-                sums = mul2(sums, pair(by, by));
-                rest = mul2(rest, pair(by, by));
-                top = most; at = to;
-            }
-            unsigned long long more = 0;   // of this step
-            if (huge(top) && top != -INFINITY) {
-#pragma unroll 1
-                for (int u = 0; u < kLines; ++u)
-                    if (line + u * a.per_beam < a.lines) {
-                        Raw8<T> y;
-                        y.read(row, (line + u * a.per_beam) * kLine + lane * 8, a.vocab, a.wide);
+            const unsigned long long scale = pair(kLog2e, kLog2e), less = pair(-at, -at);
+            unsigned long long of[kLines];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) { const float2 v = y.two(i); more = add2(more, pair(exp2_of((v.x - top) * kLog2e), exp2_of((v.y - top) * kLog2e))); }
-                    }
-            } else {
-                const unsigned long long scale = pair(kLog2e, kLog2e), less = pair(-at, -at);
-                unsigned long long of[kLines];
+            for (int u = 0; u < kLines; ++u)
 #pragma unroll
-                for (int u = 0; u < kLines; ++u)
+                for (int i = 0; i < 4; ++i) {
+                    const float2 v = x[u].two(i), e = halves(fma2(pair(v.x, v.y), scale, less));
+                    const unsigned long long term = pair(exp2_of(e.x), exp2_of(e.y));
+                    of[u] = i ? add2(of[u], term) : term;
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 v = x[u].two(i), e = halves(fma2(pair(v.x, v.y), scale, less));
-                        const unsigned long long term = pair(exp2_of(e.x), exp2_of(e.y));
-                        of[u] = i ? add2(of[u], term) : term;
-                    }
+            for (int apart = kLines / 2; apart > 0; apart /= 2)
 #pragma unroll
-                for (int apart = kLines / 2; apart > 0; apart /= 2)
-#pragma unroll
-                    for (int u = 0; u < apart; ++u) of[u] = add2(of[u], of[u + apart]);
-                more = of[0];
-            }
-            more = add2(more, rest);
-            const unsigned long long now = add2(sums, more), minus = pair(-1.f, -1.f);
+                for (int u = 0; u < apart; ++u) of[u] = add2(of[u], of[u + apart]);
+            const unsigned long long more = add2(of[0], rest), now = add2(sums, more), minus = pair(-1.f, -1.f);
             rest = fma2(fma2(sums, minus, now), minus, more);   // more - (now - sums)
             sums = now;
 #pragma unroll
             for (int u = 0; u < kLines; ++u) x[u] = next[u];
         }
-        // without a finite maximum the sum is zero or, with a NaN or an infinity among the logits, NaN
+        const float top = warp_max(best);
         const float2 v = halves(sums), r = halves(rest);
         double sum = ((double)v.x + (double)r.x) + ((double)v.y + (double)r.y);
+        // (without a finite maximum the sum is zero or, with a NaN or an infinity among the logits, NaN)
+        if (fabsf(top) > kFar && top != -INFINITY) sum = far_sum(row, part_of(share), a.lines, a.per_beam, a.vocab, a.wide, top);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         s.parts[turn][warp][lane] = part;
         s.steps[turn][warp][lane] = make_float4(best, second, third, __uint_as_float(which));
         if (turn == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         for (int o = 16; o >= a.groups; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if (lane < blocks) *cluster.map_shared_rank(&s.shares[share], lane) = Share{top, sum};
+        if (lane < blocks) *cluster.map_shared_rank(&s.shares[share], lane) = Share{top, at, sum};
         if (lane < a.groups)
             for (int r = 0; r < blocks; ++r) *cluster.map_shared_rank(&s.tops[share * a.groups + lane], r) = best;
     }
@@ -303,13 +306,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_beam_select(SelectArgs a) {
     // Every block: each beam's log-sum from its shares.
     for (int b = warp; b < a.beams; b += kWarps) {
         const Share* of = s.shares + b * a.per_beam;
-        float top = -INFINITY;
-        for (int j = lane; j < a.per_beam; j += 32) top = fmaxf(top, of[j].top);
+        float top = -INFINITY, highest = -INFINITY;
+        for (int j = lane; j < a.per_beam; j += 32) { top = fmaxf(top, of[j].top); highest = fmaxf(highest, fabsf(of[j].top) > kFar ? of[j].top : of[j].at * (1.f / kLog2e)); }
         top = warp_max(top);
-        const double base = base_of(top);
+        const double base = (double)warp_max(highest);
         double sum = 0;
 #pragma unroll 1
-        for (int j = lane; j < a.per_beam; j += 32) sum += of[j].top == -INFINITY ? of[j].sum : of[j].sum * exp2_64((base_of(of[j].top) - base) * (double)kLog2e);
+        for (int j = lane; j < a.per_beam; j += 32) {
+            const Share f = of[j];
+            const double down = fabsf(f.top) > kFar ? ((double)f.top - base) * (double)kLog2e : (double)f.at - base * (double)kLog2e;
+            sum += f.top == -INFINITY ? f.sum : f.sum * exp2_64(down);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {

@@ -51,3 +51,60 @@ def test_rows_of_random_logits(psb, t, batch, beams, vocab):
     x = torch.rand((beams, vocab), generator=g, device="cuda") * torch.linspace(0.1, 8.0, beams, device="cuda")[:, None]
     x[:, 5] = 12.0
     check(psb, x, vocab, batch, beams, t)
+
+
+# Logits far from zero, where what fp32 holds of a logit times log2(e) leaves nothing of its exponent: the same totals and the same order as in 64 bits.
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,beams,vocab", [(1, 4, 3000), (2, 5, 50_000), (160, 3, 1500)])
+@pytest.mark.parametrize("offset", [1e4, 1e6, 3.99e6, 4e6, -4e6, 1e7, -2e8, 1e9, 1.37e10, 1e11, -1e12, 1e20, -1e20, 1.37e37, 1e38, 3e38, -3e38])
+def test_far_logits(psb, t, batch, beams, vocab, offset):
+    from test_gpu_beams import check as check_all
+    g = torch.Generator(device="cuda").manual_seed(vocab + beams)
+    x = (torch.randn((batch * beams, vocab), generator=g, device="cuda") * 3 + offset).to(t)
+    s = -5 * torch.rand((batch, beams), generator=g, device="cuda")
+    check_all(psb, x, s, 7)
+    x[:, ::2] = torch.randn(x[:, ::2].shape, generator=g, device="cuda").to(t)   # half of them near zero
+    check_all(psb, x, s, 7)
+
+
+@pytest.mark.parametrize("vocab", [2000, 60_000])
+@pytest.mark.parametrize("batch", [1, 160])
+def test_logits_that_rise_through_every_range(psb, batch, vocab):
+    """From one way of holding the base to the next, up and down, within a share and between them."""
+    from test_gpu_beams import check as check_all
+    border = np.float32(4e6)
+    around = torch.from_numpy(border + np.arange(-vocab // 2, vocab - vocab // 2, dtype=np.float32) * np.float32(0.25))
+    rows = [around, -around, around.flip(0), -around.flip(0), torch.linspace(-5e6, 5e6, vocab), torch.logspace(0, 38, vocab), -torch.logspace(0, 38, vocab).flip(0),
+            torch.full((vocab,), 1e38), torch.full((vocab,), float(np.nextafter(np.float32(1e38), np.float32(2e38))))]
+    rows[-1][: vocab // 2] = 1e38
+    x = torch.stack(rows).float().cuda().repeat(batch, 1)
+    check_all(psb, x, -torch.arange(9.0, device="cuda").repeat(batch, 1) * 0.37, 12)
+
+
+def check_totals(psb, x, vocab, batch, beams):
+    """The same scores as in check(), where tokens and beams lie closer together than totals are exact: the totals, and each one's own."""
+    x64 = x.double()
+    log_sum = (x64 - x64.amax(1, keepdim=True)).exp().sum(1).log() + x64.amax(1)
+    order = torch.stack([torch.randperm(beams, generator=torch.Generator().manual_seed(i)) for i in range(batch)]).cuda()
+    scores = (log_sum[None] - x64.amax(1) - 1e-5 * order).float()
+    p, tokens = (torch.empty((batch, beams), dtype=torch.int32, device="cuda") for _ in range(2))
+    v = torch.empty((batch, beams), device="cuda")
+    psb.beam_select(x.repeat(batch, 1), scores, batch, beams, vocab, beams, p, tokens, v)
+    log_p = x64 - log_sum[:, None]
+    for i in range(batch):
+        total = scores[i].double()[:, None] + log_p
+        best = total.flatten().topk(beams)[0]
+        bound = 1e-6 + best.abs() * 2.0**-23
+        assert bool(((v[i].double() - best).abs() <= bound).all())
+        assert bool(((v[i].double() - total[p[i].long(), tokens[i].long()]).abs() <= bound).all())
+
+
+def test_slowly_rising_rows(psb):
+    """The base rises many times while what came before still makes up most of the sum."""
+    vocab, batch, beams = 100_000, 150, 16
+    x = torch.stack([torch.linspace(-d, 0, vocab, device="cuda") for d in torch.linspace(0.3, 20, beams).tolist()])
+    check_totals(psb, x, vocab, batch, beams)
+    y = torch.full((beams, vocab), -17.0, device="cuda")       # and a few logits that rise above many
+    y[:, ::9973] = torch.linspace(-16, 0, y[:, ::9973].shape[1], device="cuda")
+    y -= torch.linspace(0, 1, beams, device="cuda")[:, None]
+    check_totals(psb, y, vocab, batch, beams)
