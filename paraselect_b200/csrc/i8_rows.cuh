@@ -444,11 +444,12 @@ __global__ void __launch_bounds__(THREADS) k_i8_rows_any(RowArgs a) {
     };
     auto sum64 = [&](int i) { return (double)to_float(x[i]) + (NORM && r ? (double)to_float(r[i]) : 0.0); };
     auto value64 = [&](int i) { return NORM && w ? sum64(i) * (double)to_float(w[i]) : sum64(i); };
-    float mine = 0.f, sum = 0.f;
+    float mine = 0.f;
+    double squares = 0;   // (in fp32 a thread's 256 squares of a long row of alike values were 4e-6 off)
     bool some = false;
 #pragma unroll 2
     for (int i = begin; i < a.dim; i += kOnce * THREADS) {
-        float h[kOnce], u[kOnce];
+        float h[kOnce], u[kOnce], sum = 0.f;
         read(i, h, u);
 #pragma unroll
         for (int e = 0; e < kOnce; ++e) {
@@ -457,7 +458,9 @@ __global__ void __launch_bounds__(THREADS) k_i8_rows_any(RowArgs a) {
             mine = larger(mine, u[e]);
             some = some || h[e] != 0.f;
         }
+        if (NORM) squares += (double)sum;
     }
+    float sum = (float)squares;
     float top32 = block_reduce<THREADS>(mine, s_top, LargerOp());
     if (NORM) sum = block_reduce<THREADS>(sum, s_sum, SumOp());
     bool wild = !(top32 >= kSafeLow && top32 <= kSafeHigh) || (NORM && !(sum >= kSafeLow && sum <= kSafeHigh));
