@@ -871,6 +871,12 @@ def _call(name, *args):
         _check(status)
 
 
+def _fits(sizes):
+    """Refuses sizes beyond 32 bits, of which ctypes would pass on the lower half: `sizes` is the bitwise or of them all."""
+    if sizes >> 31 not in (0, -1):
+        raise InvalidArgument(1, "a size of 2^31 or more, or below -2^31")
+
+
 def _at(tensor):
     """Address of a device tensor, or None."""
     return None if tensor is None else tensor.data_ptr()
@@ -894,6 +900,7 @@ def _at_of(tensor, kind):
 
 def i8_encode_rows(d_rows, n, dim, d_codes, d_scales, row_stride=0, code_stride=0, device=0, stream=None):
     """8-bit codes of n rows and a scale for each: row = codes * scale.  Strides in elements (0 = the rows lie side by side)."""
+    _fits(dim)
     _call("psb_i8_encode_rows", _at(d_rows), _type(d_rows), n, dim, row_stride or dim, _at_of(d_codes, "int8"), code_stride or dim, _at_of(d_scales, "float32"), device, stream)
 
 
@@ -903,12 +910,14 @@ def i8_norm_rows(d_rows, n, dim, d_weight, eps, d_codes, d_scales, d_residual=No
     kind, dtype = _type(d_rows), d_rows.dtype
     if (d_weight is not None and d_weight.dtype != dtype) or (d_residual is not None and d_residual.dtype != dtype) or (d_sum is not None and d_sum.dtype != dtype):
         raise InvalidArgument(1, "rows, weight, residual and sum are of one type")
+    _fits(dim)
     _call("psb_i8_norm_rows", _at(d_rows), _at(d_residual), _at(d_weight), kind, n, dim, row_stride or dim, residual_stride or dim, eps,
           _at(d_sum), sum_stride or dim, _at_of(d_codes, "int8"), code_stride or dim, _at_of(d_scales, "float32"), device, stream)
 
 
 def i8_matmul(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, x_stride=0, w_stride=0, out_stride=0, device=0, stream=None):
     """out [m][n] = the products of m and n rows of k codes, with both sides' scales."""
+    _fits(k)
     _call("psb_i8_matmul", _at_of(d_x, "int8"), x_stride or k, _at_of(d_x_scales, "float32"), m, _at_of(d_w, "int8"), w_stride or k, _at_of(d_w_scales, "float32"), n, k, _at(d_out), _type(d_out),
           out_stride or n, device, stream)
 
@@ -916,18 +925,21 @@ def i8_matmul(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, x_stride=0, w_st
 def i8_matmul_limited(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, tiles=-1, polls=1 << 22, x_stride=0, w_stride=0, out_stride=0,
                       device=0, stream=None):
     """Test hook of i8_matmul's time-out path; see include/psb.h."""
+    _fits(k | polls)
     _call("psb_i8_matmul_limited", _at_of(d_x, "int8"), x_stride or k, _at_of(d_x_scales, "float32"), m, _at_of(d_w, "int8"), w_stride or k, _at_of(d_w_scales, "float32"), n, k, _at(d_out),
           _type(d_out), out_stride or n, tiles, polls, device, stream)
 
 
 def beam_select(d_logits, d_scores, batch, beams, vocab, k, d_parents, d_tokens, d_totals, row_stride=0, device=0, stream=None):
     """The k best continuations of every item over its beams and the vocabulary: parents and tokens [batch][k] int32, totals fp32."""
+    _fits(batch | beams | vocab | k)
     _call("psb_beam_select", _at(d_logits), _type(d_logits), row_stride or vocab, _at_of(d_scores, "float32"), batch, beams, vocab, k, _at_of(d_parents, "int32"),
           _at_of(d_tokens, "int32"), _at_of(d_totals, "float32"), device, stream)
 
 
 def beam_reorder(d_in, d_out, d_parents, layers, batch, beams, heads, tokens, token_bytes, d_lengths=None, device=0, stream=None):
     """States [layers][batch][beams][heads][tokens][token_bytes] in the order of the chosen parents; d_out may be d_in."""
+    _fits(layers | batch | beams | heads | tokens)
     _call("psb_beam_reorder", _at(d_in), _at(d_out), _at_of(d_parents, "int32"), layers, batch, beams, heads, tokens, token_bytes, _at_of(d_lengths, "int32"), device, stream)
 
 

@@ -140,3 +140,20 @@ def test_without_a_device_there_is_no_fallback():
     x, c, s = rows(), codes(), torch.zeros(4)
     refused(5, api.i8_encode_rows, x, 4, 32, c, s)
     refused(5, api.i8_matmul, c, s, 4, codes(8), torch.zeros(8), 8, 32, torch.zeros((4, 8)))
+
+
+def test_sizes_beyond_32_bits():
+    """They are refused, not cut to their lower half: 2^32 + 32 elements a row are not 32, 2^32 items are not none."""
+    big = 1 << 32
+    x, c, s, i = rows(), codes(), torch.zeros(4), torch.zeros((2, 3), dtype=torch.int32)
+    refused(1, api.i8_encode_rows, x, 4, big + 32, c, s, row_stride=32, code_stride=32)
+    refused(1, api.i8_norm_rows, x, 4, big + 32, None, 1e-5, c, s, row_stride=32, code_stride=32)
+    refused(1, api.i8_matmul, c, s, 4, codes(8), torch.zeros(8), 8, big + 32, torch.zeros((4, 8)), x_stride=32, w_stride=32)
+    refused(1, api.i8_matmul_limited, c, s, 4, codes(8), torch.zeros(8), 8, 32, torch.zeros((4, 8)), polls=big + 1)
+    for sizes in ((big, 3, 10, 3), (2, big + 3, 10, 3), (2, 3, big + 10, 3), (2, 3, 10, big + 3), (2, 3, 10, (1 << 31) + 3), (2, -big + 3, 10, 3)):
+        refused(1, api.beam_select, torch.zeros((6, 10)), torch.zeros((2, 3)), *sizes, i, i.clone(), torch.zeros((2, 3)), row_stride=10)
+    a = torch.zeros(240)
+    for n in range(5):
+        sizes = [1, 2, 3, 4, 5]
+        sizes[n] = big if n in (0, 1, 4) else big + sizes[n]
+        refused(1, api.beam_reorder, a, a.clone(), i, *sizes, 8)
