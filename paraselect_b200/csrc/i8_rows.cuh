@@ -125,12 +125,22 @@ __device__ __forceinline__ float warp_larger(float v) {
     return r;
 }
 
-// Blocks of MOST threads that an SM's registers shall hold.
-// (16,384 x 8,192 bf16 with norm, at full clocks and after a second at the power limit: 3 170 us and 170 to 182, 4 164 and 175 to 186, 5 216; rows that begin
-// anywhere, 200,000 x 500: 3 141, 4 160; 30,000 x 4,096 without: 4 68, 5 64.5, 6 63; fp32,
-// 100,000 x 1,000 with norm: 4 189, 5 225; 1M x 96 without, 16 elements a thread: 6 74, 7 70; 100,000 x 333: 6 34, 7 38; blocks of 512, 8,000 x 16,384 bf16 with norm: 1 235, 2 181, without 125 and 85)
+// Blocks of MOST threads that an SM's registers shall hold.  More blocks hide more of each other's waits until their registers spill.  Times in us at full clocks, and
+// where a second figure stands, after a second of calls, at the power limit, by which choices are made that differ there:
+//
+//   form (kEach, threads a block)           measured on                  blocks an SM and times
+//   24 or 32, 256, norm, whole packs        16,384 x 8,192 bf16          3: 170 / 182    4: 164 / 186   5: 216
+//   24 or 32, 256, norm, SHIFT              200,000 x 500 bf16           3: 141          4: 160
+//   24 or 32, 256, whole packs              30,000 x 4,096 bf16          4: 68           5: 64.5        6: 63
+//   32, 256, SHIFT, a part of a warp a row  1M x 101 fp16                4: 82 / 86      5: 82 / 91     6: 101 / 113
+//                                           150,000 x 701 bf16           4: 94 / 95      5: 87 / 87     6: 92 / 92
+//   32, 256, SHIFT, a block a row           30,000 x 4,001 bf16          4: 80 / 81      5: 74 / 77     6: 74 / 79
+//   12 or 16, 256, norm                     100,000 x 1,000 fp32         4: 189          5: 225
+//   12 or 16, 256, whole packs              1M x 96 fp32                 6: 74           7: 70
+//   16, 256, SHIFT                          100,000 x 333 fp32           6: 34           7: 38
+//   512 threads, whole packs                8,000 x 16,384 bf16          1: 125          2: 85    (with norm 235 and 181)
 template <int kEach, int MOST, bool NORM, bool SHIFT> constexpr int blocks_of() {
-    return MOST == 256 ? (kEach >= 24 ? (NORM ? 3 : 6) : NORM ? 4 : SHIFT ? 6 : 7) : MOST == 288 || (MOST == 512 && !(NORM && SHIFT)) ? 2 : 1;
+    return MOST == 256 ? (kEach >= 24 ? (NORM ? 3 : SHIFT ? 5 : 6) : NORM ? 4 : SHIFT ? 6 : 7) : MOST == 288 || (MOST == 512 && !(NORM && SHIFT)) ? 2 : 1;
 }
 
 // One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in
