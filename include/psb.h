@@ -644,7 +644,8 @@ psb_status psb_sign_search_candidates(int mode, const float* d_states, const flo
  * Rows held as signed 8-bit codes with one fp32 scale a row, value = code * scale: stored rows that are scored by inner products, and a
  * generating model's weights and activations.  No counterpart in the reference (its 8-bit rows are the caller's own u8 values).  All pointers
  * are DEVICE pointers on `device`; the calls are asynchronous on `stream`, allocate nothing, can be captured, and leave the current device as
- * it was.  Strides are in elements.  Outputs may not lie over other arrays unless said so.  Rows and columns behind the last are not written. */
+ * it was.  Strides are in elements.  Outputs may not lie over other arrays unless said so, an array being all from its first element to its last: rows of one array in the
+ * gaps between another's are refused too.  Rows and columns behind the last are not written. */
 enum { PSB_TYPE_F32 = 0, PSB_TYPE_F16 = 1, PSB_TYPE_BF16 = 2 };
 
 /* code = rint(127 x / max|x|), ties to even, as in 64-bit arithmetic; scale = max|x| / 127.  A row of zeros has scale 0; one with an infinity
@@ -664,7 +665,7 @@ psb_status psb_i8_norm_rows(const void* d_rows, const void* d_residual, const vo
 psb_status psb_i8_matmul(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride,
                          const float* d_w_scales, int64_t n, int k, void* d_out, int out_type, int64_t out_stride, int device, void* stream);
 /* Test hook of its time-out path: only the first `tiles` output tiles (-1: all) get their products from the tensor cores, waits end after `polls`.
- * A block that waits in vain forms its outputs without them, so that the results are the same. */
+ * A block that waits in vain, in whichever role, ends what it has under way and forms its outputs without the tensor cores, so that the results are the same. */
 psb_status psb_i8_matmul_limited(const int8_t* d_x, int64_t x_stride, const float* d_x_scales, int64_t m, const int8_t* d_w, int64_t w_stride,
                                  const float* d_w_scales, int64_t n, int k, void* d_out, int out_type, int64_t out_stride, int64_t tiles, int polls,
                                  int device, void* stream);

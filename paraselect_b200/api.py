@@ -832,6 +832,8 @@ def pq_encode_limited(d_data, n, dim, d_codebook, M, K, d_codes, items=-1, d_gav
 
 
 # ---- rows of 8-bit codes, beams -------------------------------------------------------------------------
+# Like the calls above these take a stream's handle, and without one the device's default stream, not the one that a tensor library has made current: a program that
+# works on a side stream passes it (torch: stream=torch.cuda.current_stream().cuda_stream).
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 _TYPE_NAMES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}
 _types = {}   # a tensor library's type object -> PSB_TYPE_*
@@ -899,14 +901,14 @@ def _at_of(tensor, kind):
 
 
 def i8_encode_rows(d_rows, n, dim, d_codes, d_scales, row_stride=0, code_stride=0, device=0, stream=None):
-    """8-bit codes of n rows and a scale for each: row = codes * scale.  Strides in elements (0 = the rows lie side by side)."""
+    """8-bit codes of n rows and a scale for each: row = codes * scale.  Strides in elements (0 = the rows lie side by side).  stream: a handle (None = the default stream)."""
     _fits(dim)
     _call("psb_i8_encode_rows", _at(d_rows), _type(d_rows), n, dim, row_stride or dim, _at_of(d_codes, "int8"), code_stride or dim, _at_of(d_scales, "float32"), device, stream)
 
 
 def i8_norm_rows(d_rows, n, dim, d_weight, eps, d_codes, d_scales, d_residual=None, d_sum=None, row_stride=0, residual_stride=0,
                  sum_stride=0, code_stride=0, device=0, stream=None):
-    """8-bit codes of the root-mean-square norm of rows + residual; d_sum receives the sum, and may be d_rows or d_residual."""
+    """8-bit codes of the root-mean-square norm of rows + residual; d_sum receives the sum, and may be d_rows or d_residual.  stream: a handle (None = the default stream)."""
     kind, dtype = _type(d_rows), d_rows.dtype
     if (d_weight is not None and d_weight.dtype != dtype) or (d_residual is not None and d_residual.dtype != dtype) or (d_sum is not None and d_sum.dtype != dtype):
         raise InvalidArgument(1, "rows, weight, residual and sum are of one type")
@@ -916,7 +918,7 @@ def i8_norm_rows(d_rows, n, dim, d_weight, eps, d_codes, d_scales, d_residual=No
 
 
 def i8_matmul(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, x_stride=0, w_stride=0, out_stride=0, device=0, stream=None):
-    """out [m][n] = the products of m and n rows of k codes, with both sides' scales."""
+    """out [m][n] = the products of m and n rows of k codes, with both sides' scales.  stream: a handle (None = the default stream)."""
     _fits(k)
     _call("psb_i8_matmul", _at_of(d_x, "int8"), x_stride or k, _at_of(d_x_scales, "float32"), m, _at_of(d_w, "int8"), w_stride or k, _at_of(d_w_scales, "float32"), n, k, _at(d_out), _type(d_out),
           out_stride or n, device, stream)
@@ -931,14 +933,15 @@ def i8_matmul_limited(d_x, d_x_scales, m, d_w, d_w_scales, n, k, d_out, tiles=-1
 
 
 def beam_select(d_logits, d_scores, batch, beams, vocab, k, d_parents, d_tokens, d_totals, row_stride=0, device=0, stream=None):
-    """The k best continuations of every item over its beams and the vocabulary: parents and tokens [batch][k] int32, totals fp32."""
+    """The k best continuations of every item over its beams and the vocabulary: parents and tokens [batch][k] int32, totals fp32.  stream: a handle (None = the default
+    stream)."""
     _fits(batch | beams | vocab | k)
     _call("psb_beam_select", _at(d_logits), _type(d_logits), row_stride or vocab, _at_of(d_scores, "float32"), batch, beams, vocab, k, _at_of(d_parents, "int32"),
           _at_of(d_tokens, "int32"), _at_of(d_totals, "float32"), device, stream)
 
 
 def beam_reorder(d_in, d_out, d_parents, layers, batch, beams, heads, tokens, token_bytes, d_lengths=None, device=0, stream=None):
-    """States [layers][batch][beams][heads][tokens][token_bytes] in the order of the chosen parents; d_out may be d_in."""
+    """States [layers][batch][beams][heads][tokens][token_bytes] in the order of the chosen parents; d_out may be d_in.  stream: a handle (None = the default stream)."""
     _fits(layers | batch | beams | heads | tokens)
     _call("psb_beam_reorder", _at(d_in), _at(d_out), _at_of(d_parents, "int32"), layers, batch, beams, heads, tokens, token_bytes, _at_of(d_lengths, "int32"), device, stream)
 

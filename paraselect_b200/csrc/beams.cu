@@ -491,8 +491,8 @@ template <typename T>
 psb_status select(SelectArgs a, int batch, int sms, cudaStream_t s) {
     a.lines = (a.vocab + kLine - 1) / kLine;
     a.wide = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.row_stride * sizeof(T) % 16 == 0;
-    // blocks an item: as many as fill the GPU once (two an SM), while each warp has a line.  64 x 8 x 128,000 bf16: 4 blocks 38.6 us, 3 49.6, 8 51, 9 58.7; one item of
-    // 4 x 32,000 fp32: 16 blocks 9 us
+    // blocks an item: as many as fill the GPU once (two an SM), while each warp has a line.  64 x 8 x 128,000 bf16: 4 blocks 39.7 us, 2 51.0, 8 49.0; 38 x 16 x 24,800 fp16:
+    // 4 blocks 20.4, 2 22.0, 8 25.0; one item of 4 x 32,000 fp32: 16 blocks 8.9
     int blocks = 1;
     while (blocks < kMaxCluster && (long long)batch * blocks * 2 <= 2 * sms && (long long)a.beams * a.lines >= (long long)blocks * kWarps * 2) blocks *= 2;
     const int warps = blocks * kWarps;

@@ -144,15 +144,20 @@ template <int kEach, int MOST, bool NORM, bool SHIFT> constexpr int blocks_of() 
 }
 
 // One row for each group of TPR threads of a warp, or for each block (TPR = 0, blocks of at most MOST threads), in registers: kEach elements a thread, in
-// packs of 16 bytes.  What few elements need - 64 bits next to ties, at the top, in rows out of fp32's range - is read again from memory, before the sum
-// is written, by the 32 lanes of a warp for the one that found it.  Code for it beside every element took five times the kernel's time, and a thread of its own for it half of the rest, the block waiting
-// (16,384 rows of 8,192 in bf16: 789 and 499 us).  fp32 arithmetic goes two elements an instruction: the kernel was bound by issue (239 us).
+// packs of 16 bytes.
 //
-// SHIFT: rows that begin and end anywhere.  Packs are those of memory; the elements before the row's first and behind its last, fewer than a pack each, go
-// to threads one by one, beside their packs.  The weight's packs lie otherwise: a block takes every G-th row, G a multiple of a pack's elements, so that
-// it is put in place once, in shared memory.  (7,000 rows of 8,191 in bf16 with norm and sum, element by element 317 us; with first and last packs that are
-// checked element by element, as part of every pack's code, and the weight's packs shifted anew for each row 273, put in place once 128, so 102.  Rows that
-// begin at packs lose by keeping the weight: 74 us and 82.)
+// What few elements need is done apart: 64 bits next to ties, at the top, in rows out of fp32's range.  Such an element is read again from memory, before the
+// sum is written, by the 32 lanes of a warp for the one that found it.  (16,384 rows of 8,192 in bf16 with norm: 789 us with that code beside every element, 499 with
+// a thread of its own doing it while the block waited, 239 this way.)  fp32 arithmetic then goes two elements an instruction, since the kernel was bound by issue (212).
+//
+// SHIFT: rows that begin and end anywhere.  Packs are those of memory.  The elements before the row's first pack and behind its last, fewer than a pack each, go
+// to threads one by one, beside their packs.  The weight's packs lie otherwise: a block takes every G-th row, G a multiple of a pack's elements, so that it is
+// put in place once, in shared memory.  7,000 rows of 8,191 in bf16 with norm and sum:
+//   317 us  element by element
+//   273 us  the first and last packs checked element by element within every pack's code, the weight's packs shifted anew for each row
+//   128 us  the weight put in place once
+//   102 us  the first and last elements one by one
+// Rows that begin at packs lose by keeping the weight (74 us, kept 82).
 template <typename T, int kEach, int TPR, int MOST, bool NORM, bool SHIFT>
 __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM, SHIFT>())) k_i8_rows(RowArgs a) {
     constexpr bool kBlock = TPR == 0;
@@ -407,9 +412,10 @@ __global__ void __launch_bounds__(MOST, (blocks_of<kEach, MOST, NORM, SHIFT>()))
     } while (kKeep && (kBlock ? row < a.n : __any_sync(0xffffffffu, row < a.n)));
 }
 
-// Rows too long for registers, or whose arrays begin at places that differ within a pack: a block a row, element by element, read again for the codes
-// (from L2, as a rule), four elements of a thread at once, or a pack of 16 bytes where rows are whole packs.  Each thread writes only elements it has read itself, so the sum may lie over the rows or the
-// residual.  (4,000 rows of 20,001 in fp32 with every code in 64 bits: 151 us, so 132; 2,000 of 40,000 in bf16 element by element 137, by packs 87.)
+// Rows too long for registers, or whose arrays begin at places that differ within a pack: a block a row, which is read again for the codes (from L2, as a rule).  A
+// thread takes four elements at once, THREADS apart, or a pack of 16 bytes where rows are whole packs.  Each thread writes only elements it has read itself, so the
+// sum may lie over the rows or the residual.  (Element by element and by packs, 2,000 x 40,000 bf16: 137 and 87 us.  4,000 x 20,001 fp32: 151 us with every code in
+// 64 bits, 132 with those next to ties alone.)
 template <typename T, bool NORM, int THREADS, bool PACKS>
 __global__ void __launch_bounds__(THREADS) k_i8_rows_any(RowArgs a) {
     __shared__ double s_sum64[32];
@@ -563,8 +569,8 @@ psb_status start(const RowArgs& a, int threads, int sms, cudaStream_t s) {
     return PSB_OK;
 }
 
-// TPR threads a row, each with three quarters of the elements where those hold it (at the power limit: 1M x 96 fp32 82.4 us, so 79.2; 500,000 x 96 bf16 with norm 72.7 and 66.8;
-// 60,000 x 768 68.8 and 63.8).
+// TPR threads a row, each with three quarters of the elements where those hold it.  At the power limit, with all the elements and with three quarters:
+// 1M x 96 fp32 82.4 and 79.2 us, 500,000 x 96 bf16 with norm 72.7 and 66.8, 60,000 x 768 bf16 with norm 68.8 and 63.8.
 template <typename T, int TPR, bool NORM, bool SHIFT>
 psb_status start_of(const RowArgs& a, int sms, cudaStream_t s) {
     constexpr int kMost = Pack<T>::VEC == 8 ? 32 : 16;
