@@ -676,8 +676,9 @@ psb_status psb_i8_matmul_limited(const int8_t* d_x, int64_t x_stride, const floa
 /* The k best continuations of each of `batch` items over its beams and the vocabulary: total = d_scores[item][beam] + log p(token), log p the
  * log-softmax of the beam's logits (d_logits [batch * beams][row_stride] of `type`), largest first, ties to the lowest (beam, token).  A token
  * with logit -inf is never chosen; neither is one of a beam whose score is not finite or whose logits hold a NaN or +inf or nothing but -inf.
- * A beam's sum of exponentials is formed from fp32 terms: its logarithm, the same for all of the beam's tokens, is off by less than 1e-6 for any vocabulary, so that
- * candidates of different beams whose totals lie closer together than 2e-6 may come in either order.  A beam's own tokens, and equal rows, are ordered exactly.
+ * A beam's sum of exponentials is formed from fp32 terms: its logarithm, the same for all of the beam's tokens, is off by less than 2e-6 for any vocabulary (1e-6 where
+ * the sum's larger part comes from logits within 10 of the largest), so that candidates of different beams whose totals lie closer together than 4e-6 may come in
+ * either order.  A beam's own tokens, and equal rows, are ordered exactly.
  * d_parents, d_tokens [batch][k] int32 (-1 where fewer are left), d_totals [batch][k] fp32 (-inf there).  d_totals may be
  * d_scores itself where k = beams; no other output lies over another array.  beams <= 64, k <= 64, vocab <= 2^24, batch <= 2^20. */
 psb_status psb_beam_select(const void* d_logits, int type, int64_t row_stride, const float* d_scores, int batch, int beams, int vocab, int k,

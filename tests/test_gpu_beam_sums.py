@@ -108,3 +108,21 @@ def test_slowly_rising_rows(psb):
     y[:, ::9973] = torch.linspace(-16, 0, y[:, ::9973].shape[1], device="cuda")
     y -= torch.linspace(0, 1, beams, device="cuda")[:, None]
     check_totals(psb, y, vocab, batch, beams)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("batch,vocab", [(150, 100_000), (1, 1 << 24)])
+def test_sums_of_logits_far_below_the_largest(psb, t, batch, vocab):
+    """One logit at the top, all others d below.  The exponent's rounding is then half a unit of up to 2^-19, times ln 2: 11 of the units above, and log2(e)'s for d up to
+    17 3.8 - with the rest 4 + 11 + 3.8 + 7 = 25.8, 1.54e-6."""
+    beams = 9
+    x = -torch.linspace(9.0, 17.0, beams, device="cuda")[:, None].repeat(1, vocab).to(t)
+    x[:, 7] = 0
+    log_sum = torch.log(1 + (vocab - 1) * x[:, 0].double().exp())
+    p, tokens = (torch.empty((batch, beams), dtype=torch.int32, device="cuda") for _ in range(2))
+    v = torch.empty((batch, beams), device="cuda")
+    scores = torch.zeros((batch, beams), device="cuda")
+    psb.beam_select(x.repeat(batch, 1) if batch > 1 else x, scores, batch, beams, vocab, beams, p, tokens, v)
+    assert (tokens == 7).all() and torch.equal(p.sort(1)[0], torch.arange(beams, device="cuda", dtype=torch.int32).repeat(batch, 1))
+    want = -log_sum[p.long()]
+    assert bool(((v.double() - want).abs() <= 1.54e-6 + want.abs() * 2.0**-23).all())
